@@ -40,6 +40,13 @@
  *   mie_blocks_decode <- Model.forward's embedding and blocks for one decode token
  *                        (model.py:558-562): every block plan in one call
  *
+ * and, for a serving step over a ragged batch, which the reference does not have:
+ *   mie_step_reserve, mie_step_release  block tables, slots and positions from
+ *                        lengths on the device, blocks from a device free list
+ *   mie_rope_append      rotary positions for a step's q and k, k and v stored by slot
+ *   mie_paged_extend     attention of a step's packed tokens over the pool
+ *   mie_token_logprobs   log probabilities, entropy and top alternatives of logits
+ *
  * Conventions shared by every entry point
  *   - Pointers are device pointers unless stated otherwise.  The library
  *     allocates nothing and never synchronises the device: every launch is
@@ -92,7 +99,7 @@ enum mie_status {
 
 /* Library ABI version (MIE_ABI_VERSION below). */
 int32_t mie_abi_version(void);
-#define MIE_ABI_VERSION 16
+#define MIE_ABI_VERSION 17
 
 /* Message for the last non-zero status returned on this thread ("" if none). */
 const char* mie_last_error(void);
@@ -675,6 +682,137 @@ int32_t mie_block_decode_embed(const void* plan, const int64_t* token_id, const 
  */
 int32_t mie_blocks_decode(const void* const* plans, int32_t num_plans, const int64_t* token_id,
                           const int32_t* counters, int32_t position, void* stream);
+
+/*
+ * A serving step's pages, from lengths on the device.
+ *
+ * The free blocks are a stack: free_ids[0 .. *free_count), the top last, in an
+ * array of `capacity` entries.  Sequence b holds context_lens[b] tokens in the
+ * blocks block_tables[b * table_stride ..] (table_width entries) and gets
+ * new_lens[b] more (0 for a row that takes no part).  Its new blocks,
+ *   ceil((context + new) / block_size) - ceil(context / block_size),
+ * come off the stack in the order a host allocator serving the sequences one
+ * after the other would take them, and are written to the table; no other
+ * entry is.  The step's tokens are packed sequence after sequence:
+ *   starts[b]                 exclusive prefix sums of new_lens (batch + 1)
+ *   slots[t], positions[t]    token t = starts[b] + i is at position
+ *                             p = context_lens[b] + i, in slot
+ *                             block_tables[b][p / block_size] * block_size + p % block_size
+ *   context_lens_out, free_count_out   lengths and free blocks after the step
+ * Tokens from starts[batch] up to max_tokens get slot -1 and position 0.
+ *
+ * All or nothing: *status is 0, or the first that applies of
+ *   4  a negative length, or *free_count outside [0, capacity]
+ *   2  a sequence outgrows its table row
+ *   3  more than max_tokens new tokens
+ *   1  not enough free blocks
+ * and then no block is taken: starts are all 0, slots -1, and the lengths and
+ * the count come out as they went in.
+ *
+ * free_ids is read only.  The outputs must not alias the inputs.  One launch;
+ * batch <= 8192, capacity and max_tokens <= 2^30.
+ */
+int32_t mie_step_reserve(const int32_t* free_ids, int32_t capacity, const int32_t* free_count,
+                         int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                         const int32_t* context_lens, const int32_t* new_lens, int32_t batch, int32_t block_size,
+                         int32_t max_tokens, int32_t* starts, int64_t* slots, int32_t* positions,
+                         int32_t* context_lens_out, int32_t* free_count_out, int32_t* status, void* stream);
+
+/*
+ * The other way: the ceil(context_lens[b] / block_size) blocks of every
+ * sequence with finished[b] != 0 go onto the stack, sequence after sequence in
+ * table order (free_ids is written from *free_count on), and their lengths
+ * become 0; the table entries stay.  All or nothing, *status as above (2: a
+ * length past its table row; 1: the stack would outgrow `capacity`).
+ */
+int32_t mie_step_release(int32_t* free_ids, int32_t capacity, const int32_t* free_count,
+                         const int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                         const int32_t* context_lens, const uint8_t* finished, int32_t batch, int32_t block_size,
+                         int32_t* context_lens_out, int32_t* free_count_out, int32_t* status, void* stream);
+
+/*
+ * Rotary positions for a step's packed tokens, and their K and V into the
+ * pool: for t < tokens, with p = positions[t], every head of q and k
+ *   (x1, x2) -> factor * (x1 cos a - x2 sin a, x2 cos a + x1 sin a),  a = p * frequencies[i]
+ * for the pairs i < rotary_dim / 2: dims (i, i + rotary_dim / 2), or with
+ * `interleaved` (2 i, 2 i + 1); dims from rotary_dim on are copied.  The angle
+ * is reduced in float64 (frequencies: radians per position), the rotation is
+ * float32 and rounded once.  q goes to q_out (which may be q itself); k, and v
+ * as it is, go to slot slots[t] of the pool: block slots[t] / block_size,
+ * place slots[t] % block_size.  A slot outside [0, num_blocks * block_size)
+ * stores nothing (its row of q is rotated all the same).  Two tokens of a call
+ * must not share a slot.
+ *
+ * q: num_heads heads, k and v (shared strides): num_kv_heads, the pool's.
+ * head_dim <= 1024 and rotary_dim even, 2 <= rotary_dim <= head_dim; at most
+ * 2^23 tokens and 4096 heads.  float32 or bfloat16.  One launch.
+ */
+int32_t mie_rope_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, const void* v,
+                        int64_t kv_stride_t, int64_t kv_stride_h, void* k_pool, void* v_pool,
+                        int64_t pool_stride_block, int64_t pool_stride_head, int32_t num_blocks,
+                        const int64_t* slots, const int32_t* positions, const double* frequencies,
+                        int32_t rotary_dim, int32_t interleaved, float factor, int32_t tokens, int32_t num_heads,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t block_size, void* q_out,
+                        int64_t out_stride_t, int64_t out_stride_h, int32_t dtype, void* stream);
+
+/*
+ * Log probabilities of given tokens, the entropy and the top alternatives of
+ * rows of logits: for r < rows, x = logits[r * stride ..] (vocab values),
+ * z = log sum_i exp(x_i):
+ *   logprobs[r] = x[tokens[r]] - z     (NaN for a token outside [0, vocab))
+ *   entropy[r]  = -sum_i p_i log p_i,  p_i = exp(x_i - z); p_i = 0 adds 0
+ *   top_tokens[r, j], top_logprobs[r, j], j < top: the largest values in order,
+ *     the lower index first among equals (NaN counts as the largest)
+ * in float32 from float32 or bfloat16 logits.  Values of -inf are tokens that
+ * cannot be; a row of nothing else, or with a NaN or +inf, has NaN for its
+ * log probabilities and entropy.  tokens, logprobs and entropy may be NULL (with
+ * tokens NULL there are no logprobs); top_tokens and top_logprobs when top is 0.
+ * 0 <= top <= min(vocab, 64).  The workspace is mie_token_logprobs_workspace
+ * (rows, vocab, top) bytes (0 where none is needed); nothing in it needs
+ * clearing.
+ */
+int64_t mie_token_logprobs_workspace(int32_t rows, int32_t vocab, int32_t top);
+int32_t mie_token_logprobs(const void* logits, int64_t stride, int32_t rows, int32_t vocab, const int64_t* tokens,
+                           int32_t top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens,
+                           void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream);
+
+/*
+ * Attention of a step's packed tokens over the pool, any number of new tokens
+ * per sequence (one included): tokens starts[b] .. starts[b + 1] - 1 of q are
+ * the last n_b = starts[b + 1] - starts[b] of sequence b's c_b = context_lens[b]
+ * tokens, whose K and V are in the pool already (these included).  The i-th
+ * is at position p = c_b - n_b + i and sees the keys j < c_b with
+ *   (j <= p, or j < prefix_lens[b] if prefix_lens is non-NULL)
+ *   and (j > p - window, if window > 0),
+ * and for head h, reading K/V head h / (num_heads / num_kv_heads):
+ *   s_j = scale * q . k_j;  s_j = softcap * tanh(s_j / softcap) if softcap > 0;
+ *   s_j -= slopes[h] * |p - j| if slopes (float32 [num_heads]) is non-NULL;
+ *   out = sum_j softmax(s)_j v_j       (0 for a token that sees no key)
+ * with sums, maxima and softmax in float32 and the output rounded once.  Keys
+ * that a token does not see have no part in its row, whatever they hold.
+ *
+ * tokens: rows of q and out.  Rows no sequence has are left as they were; so
+ * are a sequence's tokens from the max_new-th on.  max_context_len bounds
+ * context_lens: a longer sequence's rows are NaN, as are those that see a key
+ * whose block id lies outside the pool or its table row.  head_dim 32, 64, 96,
+ * 128 or 256; rows of q, out and the pools 16-byte aligned; float32 or
+ * bfloat16; num_heads / num_kv_heads whole and at most 128; tokens <= 2^22.
+ *
+ * One launch, or two where the context is split: the workspace is
+ * mie_paged_extend_workspace's bytes for the same arguments (negative:
+ * -MIE_ERR_*), and nothing in it needs clearing.
+ */
+int64_t mie_paged_extend_workspace(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_context_len,
+                                   int32_t window, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                   int32_t dtype);
+int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,
+                         const void* v_pool, int64_t pool_stride_block, int64_t pool_stride_head,
+                         int32_t num_blocks, const int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                         const int32_t* starts, const int32_t* context_lens, int32_t tokens, int32_t batch,
+                         int32_t max_new, int32_t max_context_len, int32_t num_heads, int32_t num_kv_heads,
+                         int32_t head_dim, int32_t block_size, float scale, float softcap, const float* slopes,
+                         int32_t window, const int32_t* prefix_lens, void* out, int64_t out_stride_t,
+                         int64_t out_stride_h, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,188 @@
+// What the kernels of mie_paged_extend share: the call, a workgroup's place in
+// it (sequence, rows, keys), scores and the softmax's steps.
+//
+// Rows.  The rows of one K/V head are its query heads' rows of every new token
+// of a sequence, token after token: row r is token r / group, head r % group,
+// group = num_heads / num_kv_heads.  Grouped heads thereby share every key
+// that is read.
+#pragma once
+
+#include <math.h>
+
+#include "gemm_tile.h"
+#include "mie_common.h"
+
+namespace mie {
+namespace extend {
+
+using gemm::f32x4;
+using gemm::u32x4;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Args {
+  const char* q;
+  const char* k_pool;
+  const char* v_pool;
+  char* out;
+  int64_t q_st, q_sh, out_st, out_sh, sblk, shead;  // bytes
+  int32_t num_blocks;
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width;
+  const int32_t* starts;
+  const int32_t* lens;
+  int32_t tokens, batch, max_new, max_len, kv_heads;
+  float scale;      // log2(e) / sqrt(D), or as the caller gave it; with a cap 2 log2(e) scale / cap
+  float cap;        // softcap * log2(e), or 0
+  float cap_ratio;  // scale / softcap (float32's tanh)
+  const float* slopes;
+  int32_t window;
+  const int32_t* prefix;
+  int32_t parts, part_keys;  // a row tile's keys in `parts` pieces of part_keys at most
+  float* ws_acc;             // [tile, kv head, part, row, D]
+  float* ws_ml;              // [tile, kv head, part, row, 2]
+  FastDiv group, bs;
+};
+
+// A workgroup's rows and keys.
+struct Place {
+  int b;                // sequence; -1: none
+  int start, count, len;  // first token in q, new tokens, context length
+  int row0, rows;       // of the sequence's rows: this tile's first one, and how many the sequence has
+  int p_first, p_last;  // positions of the tile's first and last row
+  int prefix;
+  int low, high;  // keys any row of the tile sees lie in [low, high); low is a multiple of 32
+  bool bad;       // a length past the bound
+};
+
+__device__ __forceinline__ int new_tokens(const Args& a, int b, int& start) {
+  const int s = min(max(a.starts[b], 0), a.tokens), e = min(max(a.starts[b + 1], s), a.tokens);
+  start = s;
+  return e - s;
+}
+
+// The place of row tile `tile` of the batch, ROWS rows per tile.  Every lane
+// of the wave gets the same (wave-uniform) answer.
+template <int ROWS>
+__device__ __forceinline__ Place find_place(const Args& a, int tile) {
+  Place p;
+  p.b = -1;
+  int in_seq = 0;
+  const int group = a.group.d;
+  const int lane = threadIdx.x & 63;
+  if (a.max_new * group <= ROWS) {  // at most one tile per sequence
+    p.b = tile < a.batch ? tile : -1;
+  } else {
+    int seen = 0;
+    for (int base = 0; base < a.batch; base += 64) {
+      int tiles = 0, unused;
+      if (base + lane < a.batch)
+        tiles = (min(new_tokens(a, base + lane, unused), a.max_new) * group + ROWS - 1) / ROWS;
+      int upto = tiles;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int y = __shfl_up(upto, off);
+        if (lane >= off) upto += y;
+      }
+      const uint64_t past = __ballot(seen + upto > tile);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        p.b = base + l;
+        in_seq = tile - seen - __builtin_amdgcn_readlane(upto - tiles, l);
+        break;
+      }
+      seen += __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+  p.b = __builtin_amdgcn_readfirstlane(p.b);
+  in_seq = __builtin_amdgcn_readfirstlane(in_seq);
+  if (p.b < 0) return p;
+  int n = new_tokens(a, p.b, p.start);
+  p.count = n;
+  p.len = max(a.lens[p.b], 0);
+  p.bad = p.len > a.max_len;
+  n = min(n, a.max_new);
+  p.rows = n * group;
+  p.row0 = in_seq * ROWS;
+  if (p.row0 >= p.rows) {  // a sequence without new tokens
+    p.b = -1;
+    return p;
+  }
+  const int base = p.len - p.count;
+  p.p_first = base + static_cast<int>(a.group.div(p.row0));
+  p.p_last = base + static_cast<int>(a.group.div(min(p.row0 + ROWS, p.rows) - 1));
+  p.prefix = a.prefix ? min(a.prefix[p.b], p.len) : 0;
+  p.high = min(p.len, max(p.p_last + 1, p.prefix));
+  p.low = a.window > 0 ? max(0, p.p_first - a.window + 1) & ~31 : 0;
+  if (p.bad || p.high < p.low) p.high = p.low;
+  return p;
+}
+
+// Pieces the tile's keys come in (at least one: empty rows are written too).
+__device__ __forceinline__ int parts_of(const Args& a, const Place& p) {
+  return a.parts == 1 ? 1 : max(1, (p.high - p.low + a.part_keys - 1) / a.part_keys);
+}
+
+__device__ __forceinline__ bool sees(const Args& a, const Place& p, int position, int key) {
+  return (key < p.len) & ((key <= position) | (key < p.prefix)) & ((a.window == 0) | (key > position - a.window));
+}
+// Whether every row of the tile sees every key of [k0, k1).
+__device__ __forceinline__ bool all_see(const Args& a, const Place& p, int k0, int k1) {
+  return k1 <= p.len && (k1 <= p.p_first + 1 || k1 <= p.prefix) && (a.window == 0 || k0 > p.p_last - a.window);
+}
+
+// The score's base-2 exponent from q . k; `slope` is the head's times log2(e).
+template <typename T>
+__device__ __forceinline__ float exponent(const Args& a, float dot, float slope, int position, int key) {
+  float x;
+  if (a.cap > 0.f) {
+    // tanh(x) = 1 - 2 / (exp(2 x) + 1): an absolute error of 2^-23, times the
+    // cap a few 1e-6 of the exponent, which bfloat16 does not show; float32
+    // takes the library's.
+    if constexpr (sizeof(T) == 4)
+      x = a.cap * tanhf(dot * a.cap_ratio);
+    else
+      x = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(fast_exp2(dot * a.scale) + 1.f);
+  } else {
+    x = dot * a.scale;
+  }
+  if (a.slopes) x -= slope * fabsf(static_cast<float>(position - key));
+  return x;
+}
+
+// Byte offset of a key's row in one head of the pool, from its table entry;
+// the first row, and `bad`, for an id outside the pool.
+__device__ __forceinline__ int64_t row_offset(const Args& a, int key, int32_t id, int row_bytes, bool& bad) {
+  bad = static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.num_blocks);
+  const uint32_t blk = a.bs.div(static_cast<uint32_t>(key));
+  const uint32_t slot = static_cast<uint32_t>(key) - blk * a.bs.d;
+  return bad ? 0 : id * a.sblk + static_cast<int64_t>(slot) * row_bytes;
+}
+// The table entry of a key (which is below the sequence's length).
+__device__ __forceinline__ int32_t entry_of(const Args& a, int b, int key) {
+  const int blk = static_cast<int>(a.bs.div(static_cast<uint32_t>(key)));
+  return blk < a.table_width ? a.tables[b * a.table_stride + blk] : -1;
+}
+
+// x combined over the four 16-lane groups (lanes i, i + 16, i + 32, i + 48).
+template <bool MAX>
+__device__ __forceinline__ float across_groups(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const float u = __uint_as_float(a[0]), v = __uint_as_float(a[1]);
+  x = MAX ? fmaxf(u, v) : u + v;
+  a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const float s = __uint_as_float(a[0]), t = __uint_as_float(a[1]);
+  return MAX ? fmaxf(s, t) : s + t;
+}
+
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+// The same for bfloat16: the largest magnitude in each half of the words taken.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void take_magnitudes(u16x2& most, uint32_t w) {
+  most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
+}
+__device__ __forceinline__ bool not_finite(u16x2 most) { return most.x >= 0x7f80u || most.y >= 0x7f80u; }
+
+}  // namespace extend
+}  // namespace mie

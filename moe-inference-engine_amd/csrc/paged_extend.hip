@@ -1,0 +1,529 @@
+// Attention of a step's packed tokens over the paged pool (mie_paged_extend).
+//
+// Mathematics: one pass over a row's keys with the running maximum m, sum l
+// and output o of a softmax in base 2; a block of keys with maximum m' scales
+// l and o by 2^(m - m') first.  Pieces of the same row (waves, partitions) are
+// joined the same way.
+//
+// One workgroup per (16 rows, K/V head, partition of the keys).  Its four
+// waves take every fourth block of 32 keys and merge their states in LDS once;
+// there is no barrier in the loop.  Scores are computed transposed, S^T =
+// K Q^T, so a lane holds four consecutive keys of one row - the second operand
+// of O^T = V^T P^T: the probabilities never leave their registers.  V is read
+// in rows: lane i's vector holds dims 4 i .. 4 i + 3, operand rows i of four
+// 16-row blocks (block j: dims 4 i + j).  With bfloat16 V the probabilities go
+// in as the sum of two bfloat16 values, 16 bits of significand.
+//
+// What a token does not see has no part in its row even where it is not
+// finite: a masked probability is 0, and a block in which some row masks a key
+// is multiplied key by key, skipping zeros, if its V holds a NaN or infinity
+// (0 times those would be NaN).  bfloat16 takes that way for every block with
+// such a V: an infinity times the second of the two values may be NaN.
+#include <limits.h>
+
+#include <algorithm>
+
+#include "paged_extend.h"
+
+namespace {
+
+using mie::Mem;
+using mie::extend::across_groups;
+using mie::extend::Args;
+using mie::extend::f32x4;
+using mie::extend::kLog2e;
+using mie::extend::Place;
+using mie::extend::u32x4;
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kRows = 16;
+
+// V's operands of one 64- or 32-dim group for 32 keys, and their products.
+// Lane (i, g): keys 16 t + 4 g + r (t < 2, r < 4), dims VEC i .. VEC i + VEC - 1.
+template <typename T, int VEC> struct Values;
+template <int VEC> struct Values<float, VEC> {
+  typedef float vec __attribute__((ext_vector_type(VEC)));
+  vec v[2][4];
+  __device__ __forceinline__ void load(int t, int r, const char* p) { v[t][r] = *reinterpret_cast<const vec*>(p); }
+  __device__ __forceinline__ bool not_finite() const {
+    bool any = false;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) any |= mie::extend::not_finite(v[t][r][j]);
+    return any;
+  }
+  __device__ __forceinline__ void multiply(const float (&p)[2][4], f32x4* o) const {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t][r][j], p[t][r], o[j], 0, 0, 0);
+  }
+};
+template <int VEC> struct Values<uint16_t, VEC> {
+  uint32_t v[2][4][VEC / 2];
+  __device__ __forceinline__ void load(int t, int r, const char* p) {
+    if constexpr (VEC == 4) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      v[t][r][0] = x.x;
+      v[t][r][1] = x.y;
+    } else {
+      v[t][r][0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+  }
+  __device__ __forceinline__ bool not_finite() const {
+    mie::extend::u16x2 most = {0, 0};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int w = 0; w < VEC / 2; ++w) mie::extend::take_magnitudes(most, v[t][r][w]);
+    return mie::extend::not_finite(most);
+  }
+  // Contraction slot 4 t + r of lane group g is key 16 t + 4 g + r in both operands.
+  __device__ __forceinline__ void multiply(const float (&p)[2][4], f32x4* o) const {
+    u32x4 hi, lo;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float x = p[w / 2][2 * (w % 2)], y = p[w / 2][2 * (w % 2) + 1];
+      hi[w] = mie::pack_bf16x2(x, y);
+      lo[w] = mie::pack_bf16x2(x - mie::bf16_lo(hi[w]), y - mie::bf16_hi(hi[w]));
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      u32x4 a;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t x = v[w / 2][2 * (w % 2)][j / 2], y = v[w / 2][2 * (w % 2) + 1][j / 2];
+        a[w] = __builtin_amdgcn_perm(y, x, j % 2 ? 0x07060302u : 0x05040100u);  // the two keys' dim j
+      }
+      o[j] = mie::gemm::mfma_fragment<uint16_t>(a, hi, o[j]);
+      o[j] = mie::gemm::mfma_fragment<uint16_t>(a, lo, o[j]);
+    }
+  }
+};
+
+// Dim of register r of 16-dim block n in lane group g (the layout above).
+template <int D>
+__device__ __forceinline__ int dim_of(int n, int r, int g) {
+  constexpr int G4 = D / 64;
+  return n < G4 * 4 ? n / 4 * 64 + g * 16 + r * 4 + n % 4 : G4 * 64 + (n - G4 * 4) / 2 * 32 + g * 8 + r * 2 + n % 2;
+}
+
+// grid = tiles x parts x kv_heads, the K/V head fastest.
+template <typename T, int D>
+__global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_rows_kernel(Args a) {
+  constexpr int NCH = D * static_cast<int>(sizeof(T)) / 64;  // 64-byte pieces of a row
+  constexpr int G4 = D / 64, G2 = D % 64 / 32;               // 64- and 32-dim groups
+  constexpr int NO = G4 * 4 + G2 * 2;                        // 16-dim blocks
+  constexpr int kRowBytes = D * static_cast<int>(sizeof(T));
+  __shared__ float s_max[4][kRows], s_sum[4][kRows];
+  __shared__ __align__(16) float s_out[4][kRows][D + 4];
+  __shared__ __align__(16) int64_t s_off[4][2][32];  // each wave's row offsets, this block's and the next one's
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kvh = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
+  const int part = item % a.parts, tile = item / a.parts;
+  const Place p = mie::extend::find_place<kRows>(a, tile);
+  if (p.b < 0) return;
+  const int parts = mie::extend::parts_of(a, p);
+  if (part >= parts) return;
+  const int first = p.low + part * a.part_keys;
+  const int end = parts == 1 ? p.high : min(p.high, first + a.part_keys);
+
+  // This lane's row (the last one again past the end), its head and position.
+  const int row = min(p.row0 + i, p.rows - 1);
+  const int token = a.group.div(row);
+  const int head = kvh * a.group.d + row - token * a.group.d;
+  const int position = p.len - p.count + token;
+  const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+  const char* qp = a.q + (p.start + token) * a.q_st + head * a.q_sh + g * 16;
+  u32x4 q[NCH];
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) q[c] = *reinterpret_cast<const u32x4*>(qp + c * 64);
+
+  f32x4 o[NO];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int n = 0; n < NO; ++n) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const char* k_head = a.k_pool + kvh * a.shead;
+  const char* v_head = a.v_pool + kvh * a.shead;
+  // Lanes l and l + 32 look up key l of a block (its last key again past the end).
+  auto key_at = [&](int k0) { return min(k0 + (lane & 31), end - 1); };
+  auto place_rows = [&](int k0, int32_t id, int buffer) {
+    bool bad;
+    s_off[wave][buffer][lane & 31] = mie::extend::row_offset(a, key_at(k0), id, kRowBytes, bad);
+    __builtin_amdgcn_wave_barrier();
+    return static_cast<uint32_t>(__ballot(bad));
+  };
+  u32x4 kf[2][NCH];
+  auto load_keys = [&](int buffer) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const char* rows = k_head + s_off[wave][buffer][t * 16 + i] + g * 16;
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) kf[t][c] = *reinterpret_cast<const u32x4*>(rows + c * 64);
+    }
+  };
+
+  int k0 = first + wave * 32, buffer = 0;
+  uint32_t bad_keys = 0;
+  int32_t id = -1;  // the next block's entry
+  if (k0 < end) {
+    id = mie::extend::entry_of(a, p.b, key_at(k0));
+    bad_keys = place_rows(k0, id, 0);
+    load_keys(0);
+    if (k0 + 128 < end) id = mie::extend::entry_of(a, p.b, key_at(k0 + 128));
+  }
+  for (; k0 < end; k0 += 128, buffer ^= 1) {
+    Values<T, 4> v4[G4 > 0 ? G4 : 1];
+    Values<T, 2> v2[G2 > 0 ? G2 : 1];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const char* v = v_head + s_off[wave][buffer][t * 16 + g * 4 + r];
+#pragma unroll
+        for (int n = 0; n < G4; ++n) v4[n].load(t, r, v + (n * 64 + i * 4) * sizeof(T));
+#pragma unroll
+        for (int n = 0; n < G2; ++n) v2[n].load(t, r, v + (G4 * 64 + n * 32 + i * 2) * sizeof(T));
+      }
+    f32x4 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) s[u] = mie::gemm::mfma_fragment<T>(kf[u][c], q[c], s[u]);
+    }
+    const uint32_t bad = bad_keys;
+    if (k0 + 128 < end) {
+      bad_keys = place_rows(k0 + 128, id, buffer ^ 1);
+      load_keys(buffer ^ 1);
+      if (k0 + 256 < end) id = mie::extend::entry_of(a, p.b, key_at(k0 + 256));
+    }
+    float w[2][4];
+    float top = m;
+    const bool whole = mie::extend::all_see(a, p, k0, k0 + 32);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int in_block = u * 16 + g * 4 + r, key = k0 + in_block;
+        float x = mie::extend::exponent<T>(a, s[u][r], slope, position, key);
+        if (bad) x = bad >> in_block & 1 ? NAN : x;
+        if (!whole) x = mie::extend::sees(a, p, position, key) ? x : -INFINITY;
+        w[u][r] = x;
+        top = fmaxf(top, x);
+      }
+    top = across_groups<true>(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    if (__any(top > m)) {  // a later maximum: the sums so far shrink
+      const float alpha = mie::fast_exp2(m - ref);
+      l *= alpha;
+#pragma unroll
+      for (int n = 0; n < NO; ++n) o[n] *= alpha;
+    }
+    m = top;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        w[u][r] = mie::fast_exp2(w[u][r] - ref);
+        l += w[u][r];
+      }
+    bool odd = false;
+    if (!whole || sizeof(T) == 2) {
+#pragma unroll
+      for (int n = 0; n < G4; ++n) odd |= v4[n].not_finite();
+#pragma unroll
+      for (int n = 0; n < G2; ++n) odd |= v2[n].not_finite();
+    }
+    if (__any(odd)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          for (int from = 0; from < 4; ++from) {
+            const float weight = __shfl(w[t][r], i + 16 * from);
+            const T* v = reinterpret_cast<const T*>(v_head + s_off[wave][buffer][t * 16 + from * 4 + r]);
+#pragma unroll
+            for (int n = 0; n < NO; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = Mem<T>::get(v + dim_of<D>(n, e, g));
+                o[n][e] = weight == 0.f ? o[n][e] : o[n][e] + weight * x;
+              }
+          }
+      continue;
+    }
+#pragma unroll
+    for (int n = 0; n < G4; ++n) v4[n].multiply(w, &o[n * 4]);
+#pragma unroll
+    for (int n = 0; n < G2; ++n) v2[n].multiply(w, &o[G4 * 4 + n * 2]);
+  }
+
+  // Merge the waves: the largest maximum, then the rescaled sums and outputs.
+  l = across_groups<false>(l);
+  if (g == 0) {
+    s_max[wave][i] = m;
+    s_sum[wave][i] = l;
+  }
+  __syncthreads();
+  const float top = fmaxf(fmaxf(s_max[0][i], s_max[1][i]), fmaxf(s_max[2][i], s_max[3][i]));
+  const float f = m == -INFINITY ? 1.f : mie::fast_exp2(m - top);
+  // Lane (i, g) holds, of a 64-dim group, dims 16 g + 4 r + j in o[j][r]; of a
+  // 32-dim group, dims 8 g + 2 r + j.
+#pragma unroll
+  for (int n = 0; n < G4; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const f32x4* u = &o[n * 4];
+      *reinterpret_cast<f32x4*>(&s_out[wave][i][n * 64 + g * 16 + r * 4]) =
+          f32x4{u[0][r] * f, u[1][r] * f, u[2][r] * f, u[3][r] * f};
+    }
+#pragma unroll
+  for (int n = 0; n < G2; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const f32x4* u = &o[G4 * 4 + n * 2];
+      float* dst = &s_out[wave][i][G4 * 64 + n * 32 + g * 8 + r * 2];
+      dst[0] = u[0][r] * f;
+      dst[1] = u[1][r] * f;
+    }
+  __syncthreads();
+  const int64_t piece = (static_cast<int64_t>(tile) * a.kv_heads + kvh) * a.parts + part;
+  for (int e = threadIdx.x; e < kRows * (D / 4); e += 256) {
+    const int in_tile = e / (D / 4), c = e % (D / 4) * 4;
+    const int r = p.row0 + in_tile;
+    if (r >= p.rows) break;
+    float top = s_max[0][in_tile];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, s_max[w][in_tile]);
+    float sum = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float mw = s_max[w][in_tile];
+      sum += mw == -INFINITY ? s_sum[w][in_tile] : s_sum[w][in_tile] * mie::fast_exp2(mw - top);
+      v += *reinterpret_cast<const f32x4*>(&s_out[w][in_tile][c]);
+    }
+    if (parts == 1) {
+      if (p.bad) sum = NAN;
+      v = sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v / sum;
+      const int t = a.group.div(r);
+      Mem<T>::put4(reinterpret_cast<T*>(a.out + (p.start + t) * a.out_st +
+                                        (kvh * a.group.d + r - t * a.group.d) * a.out_sh) + c, v);
+    } else {
+      *reinterpret_cast<f32x4*>(a.ws_acc + (piece * kRows + in_tile) * D + c) = v;
+      if (c == 0) {
+        a.ws_ml[(piece * kRows + in_tile) * 2] = top;
+        a.ws_ml[(piece * kRows + in_tile) * 2 + 1] = sum;
+      }
+    }
+  }
+}
+
+// Joins the partitions of a tile's rows.  grid = tiles x kv_heads.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void extend_join_kernel(Args a) {
+  const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
+  const Place p = mie::extend::find_place<kRows>(a, tile);
+  if (p.b < 0) return;
+  const int parts = mie::extend::parts_of(a, p);
+  if (parts == 1) return;
+  const int64_t piece = (static_cast<int64_t>(tile) * a.kv_heads + kvh) * a.parts;
+  for (int e = threadIdx.x; e < kRows * (D / 4); e += 256) {
+    const int in_tile = e / (D / 4), c = e % (D / 4) * 4;
+    const int r = p.row0 + in_tile;
+    if (r >= p.rows) break;
+    const float* ml = a.ws_ml + (piece * kRows + in_tile) * 2;
+    const float* acc = a.ws_acc + (piece * kRows + in_tile) * D + c;
+    float top = -INFINITY;
+    for (int j = 0; j < parts; ++j) top = fmaxf(top, ml[j * kRows * 2]);
+    float sum = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < parts; ++j) {
+      const float mj = ml[j * kRows * 2];
+      const float f = mj == -INFINITY ? 1.f : mie::fast_exp2(mj - top);
+      sum += f * ml[j * kRows * 2 + 1];
+      v += f * *reinterpret_cast<const f32x4*>(acc + static_cast<int64_t>(j) * kRows * D);
+    }
+    v = sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v / sum;
+    const int t = a.group.div(r);
+    Mem<T>::put4(reinterpret_cast<T*>(a.out + (p.start + t) * a.out_st +
+                                      (kvh * a.group.d + r - t * a.group.d) * a.out_sh) + c, v);
+  }
+}
+
+// ---- host ------------------------------------------------------------------
+
+constexpr int kMinPart = 256;       // keys of the smallest partition
+constexpr int kGroupsWanted = 1024;  // workgroups that fill the 256 CUs
+
+struct Plan {
+  int64_t tiles;
+  int parts, part_keys;
+  int64_t bytes;
+};
+
+// Row tiles: as many as the batch can have (the lengths are on the device).
+// The keys are split until the tiles make kGroupsWanted workgroups.
+Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int group, int kv_heads, int head_dim) {
+  Plan p;
+  const int64_t most = (static_cast<int64_t>(max_new) * group + kRows - 1) / kRows;
+  p.tiles = static_cast<int64_t>(max_new) * group <= kRows
+                ? batch
+                : std::min<int64_t>(batch * most, static_cast<int64_t>(tokens) * group / kRows + batch);
+  // Keys a tile can see: all, or a window back from each of its tokens.
+  const int64_t span = (kRows + group - 1) / group + 1;
+  const int64_t range = window > 0 ? std::min<int64_t>(max_len, static_cast<int64_t>(window) + span + 32) : max_len;
+  const int64_t want = std::max<int64_t>(1, kGroupsWanted / (p.tiles * kv_heads));
+  const int64_t parts = std::min<int64_t>(want, (range + kMinPart - 1) / kMinPart);
+  if (parts <= 1) {
+    p.parts = 1;
+    p.part_keys = INT_MAX;
+    p.bytes = 0;
+    return p;
+  }
+  p.part_keys = static_cast<int>(((range + parts - 1) / parts + 127) & ~127);
+  // The first key may lie up to 31 before the first one seen.
+  p.parts = static_cast<int>((range + 31 + p.part_keys - 1) / p.part_keys);
+  p.bytes = p.tiles * kv_heads * p.parts * kRows * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+  return p;
+}
+
+int32_t check_shape(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_len, int32_t window,
+                    int32_t num_heads, int32_t kv_heads, int32_t head_dim, int32_t dtype) {
+  const char* what = "mie_paged_extend";
+  if (dtype != MIE_DTYPE_F32 && dtype != MIE_DTYPE_BF16)
+    return mie::fail(MIE_ERR_UNSUPPORTED, "%s: dtype %d; float32 or bfloat16 only", what, dtype);
+  if (head_dim != 32 && head_dim != 64 && head_dim != 96 && head_dim != 128 && head_dim != 256)
+    return mie::fail(MIE_ERR_UNSUPPORTED, "%s: head_dim %d; 32, 64, 96, 128 or 256", what, head_dim);
+  if (tokens < 0 || tokens > 1 << 22 || batch < 1 || batch > 1 << 16 || max_new < 0 || max_len < 0 || max_len > 1 << 30 ||
+      window < 0)
+    return mie::fail(MIE_ERR_INVALID, "%s: bad shape tokens=%d batch=%d max_new=%d max_context_len=%d window=%d", what,
+                     tokens, batch, max_new, max_len, window);
+  if (kv_heads < 1 || num_heads < kv_heads || num_heads % kv_heads || num_heads / kv_heads > 128 || kv_heads > 1024)
+    return mie::fail(MIE_ERR_INVALID, "%s: num_heads=%d num_kv_heads=%d (at most 128 to one, 1024 of them)", what,
+                     num_heads, kv_heads);
+  return MIE_OK;
+}
+
+template <typename T, int D>
+void launch(const Args& a, const Plan& plan, hipStream_t st) {
+  extend_rows_kernel<T, D><<<static_cast<uint32_t>(plan.tiles * plan.parts * a.kv_heads), 256, 0, st>>>(a);
+  if (plan.parts > 1)
+    extend_join_kernel<T, D><<<static_cast<uint32_t>(plan.tiles * a.kv_heads), 256, 0, st>>>(a);
+}
+
+template <typename T>
+void launch_dim(const Args& a, const Plan& plan, int head_dim, hipStream_t st) {
+  switch (head_dim) {
+    case 32: launch<T, 32>(a, plan, st); break;
+    case 64: launch<T, 64>(a, plan, st); break;
+    case 96: launch<T, 96>(a, plan, st); break;
+    case 128: launch<T, 128>(a, plan, st); break;
+    default: launch<T, 256>(a, plan, st); break;
+  }
+}
+
+}  // namespace
+
+extern "C" int64_t mie_paged_extend_workspace(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_context_len,
+                                              int32_t window, int32_t num_heads, int32_t num_kv_heads,
+                                              int32_t head_dim, int32_t dtype) {
+  if (int32_t rc = check_shape(tokens, batch, max_new, max_context_len, window, num_heads, num_kv_heads, head_dim, dtype))
+    return -rc;
+  if (tokens == 0 || max_new == 0) return 0;
+  return make_plan(tokens, batch, std::min(max_new, tokens), max_context_len, window, num_heads / num_kv_heads,
+                   num_kv_heads, head_dim)
+      .bytes;
+}
+
+extern "C" int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pool,
+                                    const void* v_pool, int64_t pool_stride_block, int64_t pool_stride_head,
+                                    int32_t num_blocks, const int32_t* block_tables, int64_t table_stride,
+                                    int32_t table_width, const int32_t* starts, const int32_t* context_lens,
+                                    int32_t tokens, int32_t batch, int32_t max_new, int32_t max_context_len,
+                                    int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                    float scale, float softcap, const float* slopes, int32_t window,
+                                    const int32_t* prefix_lens, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                                    void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream) {
+  const char* what = "mie_paged_extend";
+  if (int32_t rc = check_shape(tokens, batch, max_new, max_context_len, window, num_heads, num_kv_heads, head_dim, dtype))
+    return rc;
+  if (block_size < 1 || num_blocks < 1 || table_width < 0 || table_stride < table_width)
+    return mie::fail(MIE_ERR_INVALID, "%s: block_size=%d num_blocks=%d table rows of %d, %lld apart", what, block_size,
+                     num_blocks, table_width, static_cast<long long>(table_stride));
+  if (!(softcap >= 0.f) || !(softcap < INFINITY) || !(fabsf(scale) < INFINITY))
+    return mie::fail(MIE_ERR_INVALID, "%s: scale %g, softcap %g", what, scale, softcap);
+  if (tokens == 0 || max_new == 0) return MIE_OK;
+  if (!q || !k_pool || !v_pool || !starts || !context_lens || !out || (!block_tables && table_width > 0))
+    return mie::fail(MIE_ERR_INVALID, "%s: null pointer", what);
+  if (pool_stride_head < static_cast<int64_t>(block_size) * head_dim ||
+      pool_stride_block < static_cast<int64_t>(num_kv_heads) * pool_stride_head)
+    return mie::fail(MIE_ERR_INVALID, "%s: pool strides overlap", what);
+  if (out_stride_h < head_dim || out_stride_t < head_dim)
+    return mie::fail(MIE_ERR_INVALID, "%s: rows of out overlap", what);
+  const int elt = mie::elt_size(dtype), w = 16 / elt;
+  if ((q_stride_t | q_stride_h | out_stride_t | out_stride_h | pool_stride_block | pool_stride_head) % w ||
+      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool) |
+        reinterpret_cast<uintptr_t>(out)) & 15))
+    return mie::fail(MIE_ERR_INVALID, "%s: rows of q, out and the pools must be 16-byte aligned", what);
+  max_new = std::min(max_new, tokens);
+  const int group = num_heads / num_kv_heads;
+  const Plan plan = make_plan(tokens, batch, max_new, max_context_len, window, group, num_kv_heads, head_dim);
+  if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return mie::fail(MIE_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", what,
+                     static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));
+  if (plan.tiles * plan.parts * num_kv_heads > 1 << 23)
+    return mie::fail(MIE_ERR_INVALID, "%s: %lld row tiles of %d heads are too many for a launch", what,
+                     static_cast<long long>(plan.tiles), num_kv_heads);
+  Args a;
+  a.q = static_cast<const char*>(q);
+  a.k_pool = static_cast<const char*>(k_pool);
+  a.v_pool = static_cast<const char*>(v_pool);
+  a.out = static_cast<char*>(out);
+  a.q_st = q_stride_t * elt;
+  a.q_sh = q_stride_h * elt;
+  a.out_st = out_stride_t * elt;
+  a.out_sh = out_stride_h * elt;
+  a.sblk = pool_stride_block * elt;
+  a.shead = pool_stride_head * elt;
+  a.num_blocks = num_blocks;
+  a.tables = block_tables;
+  a.table_stride = table_stride;
+  a.table_width = table_width;
+  a.starts = starts;
+  a.lens = context_lens;
+  a.tokens = tokens;
+  a.batch = batch;
+  a.max_new = max_new;
+  a.max_len = max_context_len;
+  a.kv_heads = num_kv_heads;
+  a.scale = softcap > 0.f ? 2.f * kLog2e * scale / softcap : scale * kLog2e;
+  a.cap = softcap * kLog2e;
+  a.cap_ratio = softcap > 0.f ? scale / softcap : 0.f;
+  a.slopes = slopes;
+  a.window = window;
+  a.prefix = prefix_lens;
+  a.parts = plan.parts;
+  a.part_keys = plan.part_keys;
+  a.ws_acc = static_cast<float*>(workspace);
+  a.ws_ml = a.ws_acc + plan.tiles * num_kv_heads * plan.parts * kRows * head_dim;
+  a.group = mie::FastDiv::make(static_cast<uint32_t>(group));
+  a.bs = mie::FastDiv::make(static_cast<uint32_t>(block_size));
+  mie::clear_error();
+  if (dtype == MIE_DTYPE_F32)
+    launch_dim<float>(a, plan, head_dim, static_cast<hipStream_t>(stream));
+  else
+    launch_dim<uint16_t>(a, plan, head_dim, static_cast<hipStream_t>(stream));
+  return mie::check_launch(what);
+}

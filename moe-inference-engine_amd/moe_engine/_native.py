@@ -9,6 +9,7 @@ Nothing here falls back to another implementation.  When the library is
 missing, `lib()` raises and every device entry point of the engine fails loudly.
 """
 
+import contextlib
 import ctypes
 import warnings
 from functools import lru_cache
@@ -19,7 +20,7 @@ from torch.utils._device import DeviceContext
 
 LIB_NAME = "libmie_paged.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 # enum mie_dtype
 DTYPE_CODES = {
@@ -209,6 +210,50 @@ _SIGNATURES = {
          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # logits, ids, weights, hidden, out
          _i32, _c_void_p],  # dtype, stream
     ),
+    "mie_step_reserve": (
+        _i32,
+        [_c_void_p, _i32, _c_void_p,  # free ids, their capacity, free count (device)
+         _c_void_p, _i64, _i32,  # block tables, stride, width
+         _c_void_p, _c_void_p, _i32, _i32, _i32,  # context lens, new lens, batch, block_size, max_tokens
+         _c_void_p, _c_void_p, _c_void_p,  # starts, slots (int64), positions
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p],  # context lens out, free count out, status, stream
+    ),
+    "mie_step_release": (
+        _i32,
+        [_c_void_p, _i32, _c_void_p,  # free ids, their capacity, free count (device)
+         _c_void_p, _i64, _i32,  # block tables, stride, width
+         _c_void_p, _c_void_p, _i32, _i32,  # context lens, finished (uint8), batch, block_size
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p],  # context lens out, free count out, status, stream
+    ),
+    "mie_rope_append": (
+        _i32,
+        [_c_void_p, _i64, _i64,  # q, strides t/h
+         _c_void_p, _c_void_p, _i64, _i64,  # k, v, strides t/h
+         _c_void_p, _c_void_p, _i64, _i64, _i32,  # pools, strides, num_blocks
+         _c_void_p, _c_void_p, _c_void_p, _i32, _i32, _f32,  # slots, positions, frequencies, rotary dim, interleaved, factor
+         _i32, _i32, _i32, _i32, _i32,  # tokens, heads, kv heads, head_dim, block_size
+         _c_void_p, _i64, _i64, _i32, _c_void_p],  # q out, strides t/h, dtype, stream
+    ),
+    "mie_paged_extend_workspace": (
+        _i64, [_i32] * 9),  # tokens, batch, max_new, max_context_len, window, heads, kv heads, head_dim, dtype
+    "mie_paged_extend": (
+        _i32,
+        [_c_void_p, _i64, _i64,  # q, strides t/h
+         _c_void_p, _c_void_p, _i64, _i64, _i32,  # pools, strides, num_blocks
+         _c_void_p, _i64, _i32,  # block tables, stride, width
+         _c_void_p, _c_void_p, _i32, _i32, _i32, _i32,  # starts, context lens, tokens, batch, max_new, max_context_len
+         _i32, _i32, _i32, _i32,  # heads, kv heads, head_dim, block_size
+         _f32, _f32, _c_void_p, _i32, _c_void_p,  # scale, softcap, slopes, window, prefix lens
+         _c_void_p, _i64, _i64,  # out, strides t/h
+         _c_void_p, _i64, _i32, _c_void_p],  # workspace, its bytes, dtype, stream
+    ),
+    "mie_token_logprobs_workspace": (_i64, [_i32, _i32, _i32]),  # rows, vocab, top
+    "mie_token_logprobs": (
+        _i32,
+        [_c_void_p, _i64, _i32, _i32, _c_void_p, _i32,  # logits, stride, rows, vocab, tokens (int64), top
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p,  # logprobs, entropy, top logprobs, top tokens
+         _c_void_p, _i64, _i32, _c_void_p],  # workspace, its bytes, dtype, stream
+    ),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -317,6 +362,22 @@ def stream_of(t: torch.Tensor) -> int:
     if _raw_stream is not None:
         return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def refuse_gradients(what: str, *tensors) -> None:
+    """The kernels record nothing: a call that autograd would have to follow
+    is an error, not a silent detach."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass; call it under torch.no_grad() or on detached tensors")
+
+
+def on_device_of(t: torch.Tensor):
+    """A context in which t's device is the current one, which is where a
+    launch goes; free when it already is."""
+    return _NOTHING if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_NOTHING = contextlib.nullcontext()
 
 
 def ptr(t) -> int:

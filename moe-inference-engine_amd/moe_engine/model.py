@@ -1404,3 +1404,38 @@ class Model(nn.Module):
             if cache.position >= self.max_seq_length:
                 break  # the sampled token has not entered the cache
         return out
+
+    @torch.no_grad()
+    def score(self, token_ids, top=0, cache=None):
+        """Log probabilities of a sequence's own tokens, a
+        projection.TokenLogprobs of one row for every token but the first: the
+        i-th row is the model's distribution after i + 1 tokens, at the token
+        that follows, with its entropy and its `top` likeliest tokens.  float32.
+        The sequence goes through a fresh cache (the caller's, or a contiguous
+        one) as generate's prompt does."""
+        if token_ids.dim() == 1:
+            token_ids = token_ids.unsqueeze(0)
+        token_ids = token_ids.to(self.token_embedding.weight.device).long()
+        if token_ids.shape[0] != 1:
+            raise ValueError("score() handles one sequence; use batch size 1")
+        length = token_ids.shape[1]
+        if length == 0:
+            raise ValueError("the sequence must contain at least one token")
+        if length > self.max_seq_length:
+            raise ValueError(f"sequence is {length} tokens; max_seq_length is {self.max_seq_length}")
+        most = min(self.config.vocab_size, projection.MAX_TOP_LOGPROBS)
+        if not 0 <= top <= most:
+            raise ValueError(f"top must lie in [0, {most}]")
+        if cache is None:
+            cache = self.new_cache(batch_size=1)
+        if cache.position != 0:
+            raise ValueError("score() needs a fresh cache")
+        logits = self(token_ids, cache)[0, :-1]
+        tokens = token_ids[0, 1:]
+        if _native.is_rocm_device(logits) and logits.dtype in (torch.float32, torch.bfloat16):
+            return projection.token_logprobs(logits, tokens, top=top)
+        logp = F.log_softmax(logits.float(), dim=-1)
+        # A stable sort: the lower token first among equals.
+        best = torch.sort(logits, dim=-1, descending=True, stable=True).indices[:, :top]
+        entropy = -torch.xlogy(logp.exp(), logp.exp()).sum(-1)
+        return projection.TokenLogprobs(logp.gather(1, tokens[:, None])[:, 0], entropy, logp.gather(1, best), best)

@@ -339,3 +339,113 @@ def prefill(x, cache, layer_idx, in_proj_weight, in_proj_bias, out_proj_weight, 
     if rc:
         _native.check(rc, "mie_attn_prefill")
     return out
+
+
+# Head sizes mie_paged_extend is built for.
+EXTEND_HEAD_DIMS = (32, 64, 96, 128, 256)
+
+
+def extend_batched(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    layer_idx: int,
+    block_tables: torch.Tensor,
+    starts: torch.Tensor,
+    context_lens: torch.Tensor,
+    max_new_tokens: int,
+    max_context_len: int,
+    *,
+    scale: float = None,
+    softcap: float = 0.0,
+    slopes: torch.Tensor = None,
+    window: int = 0,
+    prefix_lens: torch.Tensor = None,
+    out: torch.Tensor = None,
+) -> torch.Tensor:
+    """Attention of a step's packed tokens over the pool: chunks of prompts
+    and single decode tokens in one call, their K and V stored before it.
+
+    q [T, H, D], sequence b's tokens in rows starts[b] .. starts[b + 1] - 1
+    (int32 [B + 1]): the last of its context_lens[b] (int32 [B]) tokens.  Pools
+    [L, NB, H_kv, BS, D], H a multiple of H_kv (consecutive heads share one);
+    block_tables int32 [B, max_blocks].  max_new_tokens and max_context_len are
+    host bounds of the two lengths: a sequence's tokens past the first are left
+    out, a sequence longer than the second gets NaN.
+
+    A token at position p sees the keys j <= p of its sequence; with prefix_lens
+    (int32 [B]) also all j < prefix_lens[b]; with window > 0 only j > p - window.
+    Scores are scale * q . k (default 1 / sqrt(D)), then softcap * tanh(s /
+    softcap) if softcap > 0, then - slopes[h] * |p - j| with slopes (float32
+    [H]).  A token that sees no key gets 0.  Rows of q that no sequence has are
+    left as they are in `out` (uninitialised in a new tensor).
+
+    float32 or bfloat16, D one of EXTEND_HEAD_DIMS; float32 sums and softmax.
+    """
+    if q.dim() != 3 or k_pool.dim() != 5 or k_pool.shape != v_pool.shape:
+        raise ValueError("q must be [tokens, heads, head_dim], the pools [layers, blocks, heads, block_size, head_dim]")
+    if not 0 <= layer_idx < k_pool.shape[0]:
+        raise IndexError(f"layer {layer_idx} outside [0, {k_pool.shape[0]})")
+    tokens, heads, head_dim = q.shape
+    _, nb, kv_heads, block_size, d2 = k_pool.shape
+    if d2 != head_dim or kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"q has heads/head_dim {heads}/{head_dim}, pool has {kv_heads}/{d2}")
+    dtype, device = q.dtype, q.device
+    if k_pool.dtype != dtype or v_pool.dtype != dtype:
+        raise ValueError("q and the pools must share a dtype")
+    if not (_native.is_rocm_device(q) and k_pool.device == device and v_pool.device == device):
+        raise RuntimeError("paged attention needs q and pools on the same ROCm device")
+    if dtype not in SUPPORTED_DTYPES or head_dim not in EXTEND_HEAD_DIMS:
+        raise RuntimeError(f"extend_batched is not built for head_dim {head_dim} in {dtype}")
+    if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise ValueError("pools must be contiguous")
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.device != device \
+            or (block_tables.shape[1] > 0 and block_tables.stride(1) != 1):
+        raise ValueError("block tables must be int32 [batch, max_blocks] on q's device with unit inner stride")
+    batch = block_tables.shape[0]
+    for name, t, n in (("starts", starts, batch + 1), ("context_lens", context_lens, batch),
+                       ("prefix_lens", prefix_lens, batch)):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (n,) or t.device != device or not t.is_contiguous()):
+            raise ValueError(f"{name} must be {n} contiguous int32 values on q's device")
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (heads,) or slopes.device != device
+                               or not slopes.is_contiguous()):
+        raise ValueError(f"slopes must be {heads} contiguous float32 values on q's device")
+    max_new_tokens, max_context_len, window = int(max_new_tokens), int(max_context_len), int(window)
+    if max_new_tokens < 0 or max_context_len < 0 or window < 0:
+        raise ValueError("max_new_tokens, max_context_len and window must not be negative")
+    if not (0 <= softcap < math.inf):
+        raise ValueError(f"softcap {softcap} must be finite and not negative (0: none)")
+    _native.refuse_gradients("extend_batched", q, k_pool, v_pool, slopes)
+    if out is None:
+        out = torch.empty((tokens, heads, head_dim), dtype=dtype, device=device)
+    elif out.shape != q.shape or out.dtype != dtype or out.device != device:
+        raise ValueError(f"out must be {tuple(q.shape)} {dtype} on q's device")
+    elif out.data_ptr() == q.data_ptr() and tokens > 0:
+        raise ValueError("out must not be q")
+    if tokens == 0 or batch == 0:
+        return out
+    align = 16 // q.element_size()
+    if q.stride(2) != 1 or q.stride(0) % align or q.stride(1) % align or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    lib, code = _native.lib(), _native.dtype_code(dtype)
+    nbytes = lib.mie_paged_extend_workspace(tokens, batch, max_new_tokens, max_context_len, window, heads, kv_heads,
+                                            head_dim, code)
+    if nbytes < 0:
+        _native.check(-nbytes, "mie_paged_extend_workspace")
+    ws = _workspace(nbytes, device)
+    kl, vl = k_pool[layer_idx], v_pool[layer_idx]
+    with _native.on_device_of(q):
+        _native.check(
+            lib.mie_paged_extend(
+                q.data_ptr(), q.stride(0), q.stride(1), kl.data_ptr(), vl.data_ptr(), kl.stride(0), kl.stride(1), nb,
+                block_tables.data_ptr(), max(block_tables.stride(0), block_tables.shape[1]), block_tables.shape[1],
+                starts.data_ptr(), context_lens.data_ptr(), tokens, batch, max_new_tokens, max_context_len,
+                heads, kv_heads, head_dim, block_size, float(scale), float(softcap), _native.ptr(slopes), window,
+                _native.ptr(prefix_lens), out.data_ptr(), out.stride(0), out.stride(1),
+                _native.ptr(ws), nbytes, code, _native.stream_of(q),
+            ),
+            "mie_paged_extend",
+        )
+    return out

@@ -10,11 +10,14 @@
   row of float32 logits, in one launch.  For the logits an lm_head call with
   keep_pick=True just wrote it merges the head's per-workgroup picks
   (mie_argmax_pairs) instead of reading the row again.
+- token_logprobs (mie_token_logprobs): log probabilities of given tokens, the
+  entropy and the top alternatives of rows of logits, in one pass over them.
 
 float32 or bfloat16.
 """
 
 import threading
+from typing import NamedTuple
 
 import torch
 
@@ -215,3 +218,59 @@ def argmax(x, out=None):
 def head_workspace_bytes(vocab: int) -> int:
     """Bytes of the per-workgroup picks mie_lm_head needs for a greedy token."""
     return int(_native.lib().mie_lm_head_workspace(int(vocab)))
+
+
+class TokenLogprobs(NamedTuple):
+    """logprobs [rows] (None without tokens), entropy [rows], top_logprobs
+    [rows, top] (float32) and top_tokens [rows, top] (int64)."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor
+    top_tokens: torch.Tensor
+
+
+# The most alternatives one call gives.
+MAX_TOP_LOGPROBS = 64
+
+
+def token_logprobs(logits, tokens=None, top: int = 0) -> TokenLogprobs:
+    """log softmax of each row of logits [rows, vocab] (float32 or bfloat16
+    on a ROCm device, rows any distance apart) at tokens (int64 [rows]; NaN for
+    one outside the vocabulary), each row's entropy, and its `top` largest
+    values with their tokens, the lower token first among equals, NaN the
+    largest.  float32 results.  -inf marks a token that cannot be; a row of
+    nothing else, or with a NaN or +inf, has NaN log probabilities and entropy."""
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[1] < 1:
+        raise ValueError("logits must be [rows, vocab] in float32 or bfloat16")
+    if not _native.is_rocm_device(logits):
+        raise RuntimeError("mie_token_logprobs needs tensors on a ROCm device")
+    rows, vocab = logits.shape
+    if tokens is not None and (tokens.dtype != torch.int64 or tokens.shape != (rows,)
+                               or tokens.device != logits.device):
+        raise ValueError(f"tokens must be {rows} int64 values on the logits' device")
+    top = int(top)
+    if not 0 <= top <= min(vocab, MAX_TOP_LOGPROBS):
+        raise ValueError(f"top {top} outside [0, {min(vocab, MAX_TOP_LOGPROBS)}]")
+    _native.refuse_gradients("token_logprobs", logits)
+    if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+        logits = logits.contiguous()
+    if tokens is not None:
+        tokens = tokens.contiguous()
+    f32 = dict(dtype=torch.float32, device=logits.device)
+    logprobs = None if tokens is None else torch.empty(rows, **f32)
+    entropy, top_logprobs = torch.empty(rows, **f32), torch.empty(rows, top, **f32)
+    top_tokens = torch.empty(rows, top, dtype=torch.int64, device=logits.device)
+    lib = _native.lib()
+    nbytes = lib.mie_token_logprobs_workspace(rows, vocab, top)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+    with _native.on_device_of(logits):
+        _native.check(
+            lib.mie_token_logprobs(
+                logits.data_ptr(), max(logits.stride(0), vocab), rows, vocab, _native.ptr(tokens), top,
+                _native.ptr(logprobs), entropy.data_ptr(), top_logprobs.data_ptr(), top_tokens.data_ptr(),
+                _native.ptr(ws), nbytes, _native.dtype_code(logits.dtype), _native.stream_of(logits),
+            ),
+            "mie_token_logprobs",
+        )
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)

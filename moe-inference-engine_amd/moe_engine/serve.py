@@ -14,6 +14,9 @@ requests (temperature 0) by replaying one captured HIP graph per decode step
 (moe_engine.graphs); the graph is captured on the first such request and
 reused by every later one.  Other requests take Model.generate.
 
+Another: POST /score returns the log probabilities of a text's own tokens, the
+entropy at each and, with `top`, the likeliest alternatives (Model.score).
+
 Differences forced by this environment:
   * --checkpoint loads the reference's checkpoint format
     ({"model", "model_config", "step", ...}, read with weights_only=True,
@@ -28,6 +31,7 @@ Differences forced by this environment:
 
 import argparse
 import json
+import math
 import threading
 import time
 from pathlib import Path
@@ -72,6 +76,18 @@ class GenerateRequest(BaseModel):
     prompt_ids: Optional[List[int]] = None
     max_new_tokens: int = Field(64, ge=1)
     temperature: float = Field(0.8, ge=0.0, allow_inf_nan=False)
+
+    @model_validator(mode="after")
+    def _needs_a_prompt(self):
+        if not self.prompt and not self.prompt_ids:
+            raise ValueError("prompt or prompt_ids must be non-empty")
+        return self
+
+
+class ScoreRequest(BaseModel):
+    prompt: str = Field("", max_length=1_000_000)
+    prompt_ids: Optional[List[int]] = None
+    top: int = Field(0, ge=0, le=20)
 
     @model_validator(mode="after")
     def _needs_a_prompt(self):
@@ -137,8 +153,8 @@ def load_model(args, device_name):
     return net.to(device_name).eval(), meta
 
 
-@app.post("/generate")
-def generate(req: GenerateRequest):
+def request_ids(req) -> List[int]:
+    """The request's token ids; HTTP 400 for what the model cannot take."""
     ids = req.prompt_ids if req.prompt_ids else enc.encode(req.prompt)
     if len(ids) == 0:
         raise HTTPException(status_code=400, detail="prompt tokenizes to zero tokens")
@@ -150,6 +166,12 @@ def generate(req: GenerateRequest):
     vocab = model.config.vocab_size
     if any(not 0 <= i < vocab for i in ids):
         raise HTTPException(status_code=400, detail=f"token ids must lie in [0, {vocab})")
+    return ids
+
+
+@app.post("/generate")
+def generate(req: GenerateRequest):
+    ids = request_ids(req)
     prompt_ids = torch.tensor(ids, device=device)
 
     with generate_lock:
@@ -178,6 +200,32 @@ def generate(req: GenerateRequest):
         "new_tokens": len(new_ids),
         "finish_reason": finish_reason,
         "tokens_per_sec": round(len(new_ids) / elapsed, 1) if elapsed > 0 else None,
+    }
+
+
+@app.post("/score")
+def score(req: ScoreRequest):
+    """One entry per token: its log probability given those before it (null
+    for the first), the entropy there and the `top` likeliest tokens."""
+    ids = request_ids(req)
+    top = min(req.top, model.config.vocab_size)
+    with generate_lock:
+        cache = new_request_cache()
+        try:
+            r = model.score(torch.tensor(ids, device=device), top=top, cache=cache)
+            logprobs, entropy, top_logprobs, top_tokens = (t.tolist() for t in r)
+        finally:
+            release_request_cache(cache)
+
+    def number(x):  # JSON has no infinities
+        return x if math.isfinite(x) else None
+
+    return {
+        "token_ids": ids,
+        "logprobs": [None] + [number(x) for x in logprobs],
+        "entropy": [None] + [number(x) for x in entropy],
+        "top": [[]] + [[{"token_id": i, "logprob": number(x)} for i, x in zip(t, p)]
+                       for t, p in zip(top_tokens, top_logprobs)],
     }
 
 
