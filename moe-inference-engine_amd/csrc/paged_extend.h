@@ -19,6 +19,8 @@ using gemm::f32x4;
 using gemm::u32x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kFewRows = 16;    // rows per workgroup where a sequence has few (extend_rows_kernel)
+constexpr int kTileRows = 128;  // and where it has many (extend_tile_kernel)
 
 struct Args {
   const char* q;
@@ -39,6 +41,7 @@ struct Args {
   const float* slopes;
   int32_t window;
   const int32_t* prefix;
+  int32_t tiles;             // row tiles of the launch, a bound
   int32_t parts, part_keys;  // a row tile's keys in `parts` pieces of part_keys at most
   float* ws_acc;             // [tile, kv head, part, row, D]
   float* ws_ml;              // [tile, kv head, part, row, 2]
@@ -125,7 +128,8 @@ __device__ __forceinline__ int parts_of(const Args& a, const Place& p) {
 }
 
 __device__ __forceinline__ bool sees(const Args& a, const Place& p, int position, int key) {
-  return (key < p.len) & ((key <= position) | (key < p.prefix)) & ((a.window == 0) | (key > position - a.window));
+  return static_cast<int>(key < p.len) & (static_cast<int>(key <= position) | static_cast<int>(key < p.prefix)) &
+         (static_cast<int>(a.window == 0) | static_cast<int>(key > position - a.window));
 }
 // Whether every row of the tile sees every key of [k0, k1).
 __device__ __forceinline__ bool all_see(const Args& a, const Place& p, int k0, int k1) {
@@ -152,17 +156,18 @@ __device__ __forceinline__ float exponent(const Args& a, float dot, float slope,
 }
 
 // Byte offset of a key's row in one head of the pool, from its table entry;
-// the first row, and `bad`, for an id outside the pool.
+// for an id outside the pool a row of block 0, and `bad`.
 __device__ __forceinline__ int64_t row_offset(const Args& a, int key, int32_t id, int row_bytes, bool& bad) {
   bad = static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.num_blocks);
   const uint32_t blk = a.bs.div(static_cast<uint32_t>(key));
   const uint32_t slot = static_cast<uint32_t>(key) - blk * a.bs.d;
-  return bad ? 0 : id * a.sblk + static_cast<int64_t>(slot) * row_bytes;
+  return (bad ? 0 : id) * a.sblk + static_cast<int64_t>(slot) * row_bytes;
 }
-// The table entry of a key (which is below the sequence's length).
+// The table entry of a key (which is below the sequence's length); -1 past the row.
 __device__ __forceinline__ int32_t entry_of(const Args& a, int b, int key) {
   const int blk = static_cast<int>(a.bs.div(static_cast<uint32_t>(key)));
-  return blk < a.table_width ? a.tables[b * a.table_stride + blk] : -1;
+  const int32_t id = a.tables[b * a.table_stride + min(blk, a.table_width - 1)];
+  return blk < a.table_width ? id : -1;
 }
 
 // x combined over the four 16-lane groups (lanes i, i + 16, i + 32, i + 48).
@@ -183,6 +188,9 @@ __device__ __forceinline__ void take_magnitudes(u16x2& most, uint32_t w) {
   most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
 }
 __device__ __forceinline__ bool not_finite(u16x2 most) { return most.x >= 0x7f80u || most.y >= 0x7f80u; }
+
+// Launches extend_tile_kernel (float32 or bfloat16, the head_dims checked).
+void launch_tiles(const Args& a, int dtype, int head_dim, hipStream_t stream);
 
 }  // namespace extend
 }  // namespace mie

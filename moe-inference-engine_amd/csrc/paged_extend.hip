@@ -31,12 +31,14 @@ using mie::Mem;
 using mie::extend::across_groups;
 using mie::extend::Args;
 using mie::extend::f32x4;
+using mie::extend::kFewRows;
 using mie::extend::kLog2e;
+using mie::extend::kTileRows;
 using mie::extend::Place;
 using mie::extend::u32x4;
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kRows = 16;
+constexpr int kRows = mie::extend::kFewRows;
 
 // V's operands of one 64- or 32-dim group for 32 keys, and their products.
 // Lane (i, g): keys 16 t + 4 g + r (t < 2, r < 4), dims VEC i .. VEC i + VEC - 1.
@@ -330,30 +332,30 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_rows
   }
 }
 
-// Joins the partitions of a tile's rows.  grid = tiles x kv_heads.
-template <typename T, int D>
+// Joins the partitions of 16 of a tile's ROWS rows.  grid = (tiles x kv_heads, ROWS / 16).
+template <typename T, int D, int ROWS>
 __global__ __launch_bounds__(256) void extend_join_kernel(Args a) {
   const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
-  const Place p = mie::extend::find_place<kRows>(a, tile);
+  const Place p = mie::extend::find_place<ROWS>(a, tile);
   if (p.b < 0) return;
   const int parts = mie::extend::parts_of(a, p);
   if (parts == 1) return;
   const int64_t piece = (static_cast<int64_t>(tile) * a.kv_heads + kvh) * a.parts;
-  for (int e = threadIdx.x; e < kRows * (D / 4); e += 256) {
-    const int in_tile = e / (D / 4), c = e % (D / 4) * 4;
+  for (int e = threadIdx.x; e < 16 * (D / 4); e += 256) {
+    const int in_tile = blockIdx.y * 16 + e / (D / 4), c = e % (D / 4) * 4;
     const int r = p.row0 + in_tile;
     if (r >= p.rows) break;
-    const float* ml = a.ws_ml + (piece * kRows + in_tile) * 2;
-    const float* acc = a.ws_acc + (piece * kRows + in_tile) * D + c;
+    const float* ml = a.ws_ml + (piece * ROWS + in_tile) * 2;
+    const float* acc = a.ws_acc + (piece * ROWS + in_tile) * D + c;
     float top = -INFINITY;
-    for (int j = 0; j < parts; ++j) top = fmaxf(top, ml[j * kRows * 2]);
+    for (int j = 0; j < parts; ++j) top = fmaxf(top, ml[j * ROWS * 2]);
     float sum = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < parts; ++j) {
-      const float mj = ml[j * kRows * 2];
+      const float mj = ml[j * ROWS * 2];
       const float f = mj == -INFINITY ? 1.f : mie::fast_exp2(mj - top);
-      sum += f * ml[j * kRows * 2 + 1];
-      v += f * *reinterpret_cast<const f32x4*>(acc + static_cast<int64_t>(j) * kRows * D);
+      sum += f * ml[j * ROWS * 2 + 1];
+      v += f * *reinterpret_cast<const f32x4*>(acc + static_cast<int64_t>(j) * ROWS * D);
     }
     v = sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v / sum;
     const int t = a.group.div(r);
@@ -368,6 +370,7 @@ constexpr int kMinPart = 256;       // keys of the smallest partition
 constexpr int kGroupsWanted = 1024;  // workgroups that fill the 256 CUs
 
 struct Plan {
+  int rows;  // of a tile
   int64_t tiles;
   int parts, part_keys;
   int64_t bytes;
@@ -377,12 +380,13 @@ struct Plan {
 // The keys are split until the tiles make kGroupsWanted workgroups.
 Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int group, int kv_heads, int head_dim) {
   Plan p;
-  const int64_t most = (static_cast<int64_t>(max_new) * group + kRows - 1) / kRows;
-  p.tiles = static_cast<int64_t>(max_new) * group <= kRows
+  const int rows = p.rows = static_cast<int64_t>(max_new) * group >= 64 ? kTileRows : kFewRows;
+  const int64_t most = (static_cast<int64_t>(max_new) * group + rows - 1) / rows;
+  p.tiles = static_cast<int64_t>(max_new) * group <= rows
                 ? batch
-                : std::min<int64_t>(batch * most, static_cast<int64_t>(tokens) * group / kRows + batch);
+                : std::min<int64_t>(batch * most, static_cast<int64_t>(tokens) * group / rows + batch);
   // Keys a tile can see: all, or a window back from each of its tokens.
-  const int64_t span = (kRows + group - 1) / group + 1;
+  const int64_t span = (rows + group - 1) / group + 1;
   const int64_t range = window > 0 ? std::min<int64_t>(max_len, static_cast<int64_t>(window) + span + 32) : max_len;
   const int64_t want = std::max<int64_t>(1, kGroupsWanted / (p.tiles * kv_heads));
   const int64_t parts = std::min<int64_t>(want, (range + kMinPart - 1) / kMinPart);
@@ -395,7 +399,7 @@ Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int 
   p.part_keys = static_cast<int>(((range + parts - 1) / parts + 127) & ~127);
   // The first key may lie up to 31 before the first one seen.
   p.parts = static_cast<int>((range + 31 + p.part_keys - 1) / p.part_keys);
-  p.bytes = p.tiles * kv_heads * p.parts * kRows * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+  p.bytes = p.tiles * kv_heads * p.parts * rows * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
   return p;
 }
 
@@ -418,9 +422,16 @@ int32_t check_shape(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_
 
 template <typename T, int D>
 void launch(const Args& a, const Plan& plan, hipStream_t st) {
-  extend_rows_kernel<T, D><<<static_cast<uint32_t>(plan.tiles * plan.parts * a.kv_heads), 256, 0, st>>>(a);
-  if (plan.parts > 1)
-    extend_join_kernel<T, D><<<static_cast<uint32_t>(plan.tiles * a.kv_heads), 256, 0, st>>>(a);
+  const uint32_t rows = static_cast<uint32_t>(plan.tiles * a.kv_heads);
+  if (plan.rows == kFewRows)
+    extend_rows_kernel<T, D><<<rows * plan.parts, 256, 0, st>>>(a);
+  else
+    mie::extend::launch_tiles(a, sizeof(T) == 4 ? MIE_DTYPE_F32 : MIE_DTYPE_BF16, D, st);
+  if (plan.parts == 1) return;
+  if (plan.rows == kFewRows)
+    extend_join_kernel<T, D, kFewRows><<<dim3(rows), 256, 0, st>>>(a);
+  else
+    extend_join_kernel<T, D, kTileRows><<<dim3(rows, kTileRows / 16), 256, 0, st>>>(a);
 }
 
 template <typename T>
@@ -459,13 +470,13 @@ extern "C" int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q
   const char* what = "mie_paged_extend";
   if (int32_t rc = check_shape(tokens, batch, max_new, max_context_len, window, num_heads, num_kv_heads, head_dim, dtype))
     return rc;
-  if (block_size < 1 || num_blocks < 1 || table_width < 0 || table_stride < table_width)
+  if (block_size < 1 || num_blocks < 1 || table_width < 1 || table_stride < table_width)
     return mie::fail(MIE_ERR_INVALID, "%s: block_size=%d num_blocks=%d table rows of %d, %lld apart", what, block_size,
                      num_blocks, table_width, static_cast<long long>(table_stride));
   if (!(softcap >= 0.f) || !(softcap < INFINITY) || !(fabsf(scale) < INFINITY))
     return mie::fail(MIE_ERR_INVALID, "%s: scale %g, softcap %g", what, scale, softcap);
   if (tokens == 0 || max_new == 0) return MIE_OK;
-  if (!q || !k_pool || !v_pool || !starts || !context_lens || !out || (!block_tables && table_width > 0))
+  if (!q || !k_pool || !v_pool || !starts || !context_lens || !out || !block_tables)
     return mie::fail(MIE_ERR_INVALID, "%s: null pointer", what);
   if (pool_stride_head < static_cast<int64_t>(block_size) * head_dim ||
       pool_stride_block < static_cast<int64_t>(num_kv_heads) * pool_stride_head)
@@ -514,10 +525,11 @@ extern "C" int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q
   a.slopes = slopes;
   a.window = window;
   a.prefix = prefix_lens;
+  a.tiles = static_cast<int32_t>(plan.tiles);
   a.parts = plan.parts;
   a.part_keys = plan.part_keys;
   a.ws_acc = static_cast<float*>(workspace);
-  a.ws_ml = a.ws_acc + plan.tiles * num_kv_heads * plan.parts * kRows * head_dim;
+  a.ws_ml = a.ws_acc + plan.tiles * num_kv_heads * plan.parts * plan.rows * head_dim;
   a.group = mie::FastDiv::make(static_cast<uint32_t>(group));
   a.bs = mie::FastDiv::make(static_cast<uint32_t>(block_size));
   mie::clear_error();

@@ -400,7 +400,7 @@ def extend_batched(
     if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError("pools must be contiguous")
     if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.device != device \
-            or (block_tables.shape[1] > 0 and block_tables.stride(1) != 1):
+            or block_tables.shape[1] < 1 or block_tables.stride(1) != 1:
         raise ValueError("block tables must be int32 [batch, max_blocks] on q's device with unit inner stride")
     batch = block_tables.shape[0]
     for name, t, n in (("starts", starts, batch + 1), ("context_lens", context_lens, batch),
