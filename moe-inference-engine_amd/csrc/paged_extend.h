@@ -45,6 +45,7 @@ struct Args {
   int32_t parts, part_keys;  // a row tile's keys in `parts` pieces of part_keys at most
   float* ws_acc;             // [tile, kv head, part, row, D]
   float* ws_ml;              // [tile, kv head, part, row, 2]
+  int32_t whole_blocks;      // blocks hold a multiple of 16 keys
   FastDiv group, bs;
 };
 
@@ -127,32 +128,38 @@ __device__ __forceinline__ int parts_of(const Args& a, const Place& p) {
   return a.parts == 1 ? 1 : max(1, (p.high - p.low + a.part_keys - 1) / a.part_keys);
 }
 
-__device__ __forceinline__ bool sees(const Args& a, const Place& p, int position, int key) {
-  return static_cast<int>(key < p.len) & (static_cast<int>(key <= position) | static_cast<int>(key < p.prefix)) &
-         (static_cast<int>(a.window == 0) | static_cast<int>(key > position - a.window));
+// The keys a token sees are [low, high): those up to its own position or the
+// prefix's end, from the window's first on.
+struct Range {
+  int low, high;
+};
+__device__ __forceinline__ Range keys_of(const Args& a, const Place& p, int position) {
+  return Range{a.window > 0 ? max(0, position - a.window + 1) : 0, min(p.len, max(position + 1, p.prefix))};
 }
-// Whether every row of the tile sees every key of [k0, k1).
-__device__ __forceinline__ bool all_see(const Args& a, const Place& p, int k0, int k1) {
-  return k1 <= p.len && (k1 <= p.p_first + 1 || k1 <= p.prefix) && (a.window == 0 || k0 > p.p_last - a.window);
+// The keys every row of two positions and those between them sees.
+__device__ __forceinline__ Range shared_keys(const Args& a, const Place& p, int first, int last) {
+  return Range{keys_of(a, p, last).low, keys_of(a, p, first).high};
+}
+__device__ __forceinline__ bool holds(Range r, int k0, int k1) { return k0 >= r.low && k1 <= r.high; }
+__device__ __forceinline__ bool holds(Range r, int key) {
+  return static_cast<uint32_t>(key - r.low) < static_cast<uint32_t>(max(r.high - r.low, 0));
 }
 
-// The score's base-2 exponent from q . k; `slope` is the head's times log2(e).
+// cap tanh(q . k scale / softcap) in base 2 (Args: cap, scale, cap_ratio).
+// tanh(x) = 1 - 2 / (exp(2 x) + 1) has an absolute error of 2^-23, times the
+// cap a few 1e-6 of the exponent, which bfloat16 does not show; float32 takes
+// the library's.
 template <typename T>
-__device__ __forceinline__ float exponent(const Args& a, float dot, float slope, int position, int key) {
-  float x;
-  if (a.cap > 0.f) {
-    // tanh(x) = 1 - 2 / (exp(2 x) + 1): an absolute error of 2^-23, times the
-    // cap a few 1e-6 of the exponent, which bfloat16 does not show; float32
-    // takes the library's.
-    if constexpr (sizeof(T) == 4)
-      x = a.cap * tanhf(dot * a.cap_ratio);
-    else
-      x = a.cap - 2.f * a.cap * __builtin_amdgcn_rcpf(fast_exp2(dot * a.scale) + 1.f);
-  } else {
-    x = dot * a.scale;
-  }
-  if (a.slopes) x -= slope * fabsf(static_cast<float>(position - key));
-  return x;
+__device__ __forceinline__ float capped(float dot, float cap, float scale, float ratio) {
+  if constexpr (sizeof(T) == 4) return cap * tanhf(dot * ratio);
+  return fmaf(-2.f * cap, __builtin_amdgcn_rcpf(fast_exp2(dot * scale) + 1.f), cap);
+}
+// The score's base-2 exponent from q . k; `slope` is the head's times log2(e),
+// `away` the position less the key's.
+template <typename T>
+__device__ __forceinline__ float exponent(const Args& a, float dot, float slope, float away) {
+  const float x = a.cap > 0.f ? capped<T>(dot, a.cap, a.scale, a.cap_ratio) : dot * a.scale;
+  return a.slopes ? fmaf(-slope, fabsf(away), x) : x;
 }
 
 // Byte offset of a key's row in one head of the pool, from its table entry;

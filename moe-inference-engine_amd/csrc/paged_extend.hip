@@ -145,6 +145,8 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_rows
   const int head = kvh * a.group.d + row - token * a.group.d;
   const int position = p.len - p.count + token;
   const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
+  const mie::extend::Range keys = mie::extend::keys_of(a, p, position);
+  const mie::extend::Range shared = mie::extend::shared_keys(a, p, p.p_first, p.p_last);
   const char* qp = a.q + (p.start + token) * a.q_st + head * a.q_sh + g * 16;
   u32x4 q[NCH];
 #pragma unroll
@@ -212,15 +214,15 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_rows
     }
     float w[2][4];
     float top = m;
-    const bool whole = mie::extend::all_see(a, p, k0, k0 + 32);
+    const bool whole = mie::extend::holds(shared, k0, k0 + 32);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int in_block = u * 16 + g * 4 + r, key = k0 + in_block;
-        float x = mie::extend::exponent<T>(a, s[u][r], slope, position, key);
+        float x = mie::extend::exponent<T>(a, s[u][r], slope, static_cast<float>(position - key));
         if (bad) x = bad >> in_block & 1 ? NAN : x;
-        if (!whole) x = mie::extend::sees(a, p, position, key) ? x : -INFINITY;
+        if (!whole) x = mie::extend::holds(keys, key) ? x : -INFINITY;
         w[u][r] = x;
         top = fmaxf(top, x);
       }
@@ -525,6 +527,7 @@ extern "C" int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q
   a.slopes = slopes;
   a.window = window;
   a.prefix = prefix_lens;
+  a.whole_blocks = block_size % 16 == 0;
   a.tiles = static_cast<int32_t>(plan.tiles);
   a.parts = plan.parts;
   a.part_keys = plan.part_keys;

@@ -62,8 +62,10 @@ __device__ __forceinline__ int value_swizzle(int key) {
 }
 
 // A value the compiler must take as new here: what is computed from it in a
-// rare path stays there instead of being kept in registers across the loop.
-__device__ __forceinline__ int fresh(int x) {
+// rare path stays there, neither kept in registers across the loop nor done on
+// every path.
+template <typename X>
+__device__ __forceinline__ X fresh(X x) {
   asm volatile("" : "+v"(x));
   return x;
 }
@@ -106,8 +108,9 @@ struct Tile {
   static constexpr int CH = kRowBytes / 16;
   static constexpr int kBytes = KT * kRowBytes;
   static constexpr int kLoads = kBytes / 4096;  // 16-byte loads per lane for K, and as many for V
+  static constexpr int kKeys = KT / 4;          // keys a wave loads
   static constexpr int NQ = D / Products<T>::kDims, NB = KT / 32, ND = D / 32;
-  static_assert(kBytes % 4096 == 0, "a tile divides among four waves");
+  static_assert(kBytes % 4096 == 0 && 16 % kKeys == 0, "a tile divides among four waves");
 };
 
 // Where a lane reads in a tile.  XORs touch the bits below a row only, so an
@@ -148,7 +151,8 @@ struct State {
   float m, l;  // m: what the sums are relative to; l: this lane's half of the keys
   int position, row_head;
   float slope;
-  int p_first, p_last, low, high;  // the wave's rows: positions, and the keys they see
+  mie::extend::Range keys;         // this row sees
+  mie::extend::Range some, shared;  // some / every row of the wave sees
 };
 
 template <typename T, int D>
@@ -235,12 +239,14 @@ template <typename T, int D>
 __device__ __attribute__((noinline)) void mend_rows(Args a, Place p, const char* v_head, int first, int end, int position, bool odd, f32x4* out, float& sum) {
   using L = Tile<T, D>;
   const int h = (threadIdx.x & 63) >> 5;
+  const mie::extend::Range keys = mie::extend::keys_of(a, p, position);
+  const mie::extend::Range shared = mie::extend::shared_keys(a, p, p.p_first, p.p_last);
   for (int k0 = first; k0 < end; k0 += L::KT) {
-    const bool whole = mie::extend::all_see(a, p, k0, k0 + L::KT);
+    const bool whole = mie::extend::holds(shared, k0, k0 + L::KT);
     for (int key = k0; key < min(k0 + L::KT, end); ++key) {
       bool bad;
       const int64_t off = mie::extend::row_offset(a, key, mie::extend::entry_of(a, p.b, key), L::kRowBytes, bad);
-      const bool seen = mie::extend::sees(a, p, position, key);
+      const bool seen = mie::extend::holds(keys, key);
       if (bad && seen) sum = NAN;
       if (bad || whole || !odd) continue;
       const T* v = reinterpret_cast<const T*>(v_head + off);
@@ -254,7 +260,7 @@ __device__ __attribute__((noinline)) void mend_rows(Args a, Place p, const char*
 }
 
 template <typename T, int D>
-__device__ __forceinline__ void attend(const Args& a, const Place& p, State<T, D>& w, const Reads<T, D>& at,
+__device__ __forceinline__ void attend(const Args& a, State<T, D>& w, const Reads<T, D>& at,
                                        const char* k_tile, const char* v_tile, int k0) {
   using L = Tile<T, D>;
   f32x16 s[L::NB];
@@ -266,23 +272,38 @@ __device__ __forceinline__ void attend(const Args& a, const Place& p, State<T, D
     for (int c = 0; c < L::NQ; ++c)
       s[b] = Products<T>::scores(*reinterpret_cast<const u32x4*>(k_tile + at.key(b, c)), w.q[c], s[b]);
   }
-  const bool whole = k0 + L::KT <= p.len && (k0 + L::KT <= w.p_first + 1 || k0 + L::KT <= p.prefix) &&
-                     (a.window == 0 || k0 > w.p_last - a.window);
-  float top = -INFINITY, scale = 1.f;
-  if (whole && a.cap == 0.f && !a.slopes && a.scale > 0.f) {
-    // The scale goes into the exponential's operand.
-    scale = a.scale;
-  } else {
-    const int key0 = fresh(k0 + 4 * ((threadIdx.x & 63) >> 5));
+  float top = -INFINITY, scale = a.scale;  // a positive scale goes into the exponential's operand
+  const int key0 = fresh(k0 + 4 * ((threadIdx.x & 63) >> 5));
+  if (a.cap > 0.f || a.slopes || !(a.scale > 0.f)) {
+    const float dot_scale = fresh(a.scale);
+    scale = 1.f;
+    if (a.cap > 0.f) {
+      const float cap = fresh(a.cap);
+#pragma unroll
+      for (int b = 0; b < L::NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[b][i] = mie::extend::capped<T>(s[b][i], cap, dot_scale, a.cap_ratio);
+    } else {
+#pragma unroll
+      for (int b = 0; b < L::NB; ++b) s[b] *= dot_scale;
+    }
+    if (a.slopes) {
+      const float away = fresh(static_cast<float>(w.position - key0));
+#pragma unroll
+      for (int b = 0; b < L::NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[b][i] = fmaf(-w.slope, fabsf(away - static_cast<float>(b * 32 + in_block(i, 0))), s[b][i]);
+    }
+  }
+  if (!mie::extend::holds(w.shared, k0, k0 + L::KT)) {
+    const mie::extend::Range seen{fresh(w.keys.low - key0), w.keys.high - key0};
 #pragma unroll
     for (int b = 0; b < L::NB; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = key0 + b * 32 + in_block(i, 0);
-        const float x = mie::extend::exponent<T>(a, s[b][i], w.slope, w.position, key);
-        const int seen = static_cast<int>(whole) | static_cast<int>(mie::extend::sees(a, p, w.position, key));
-        s[b][i] = seen ? x : -INFINITY;
-      }
+      for (int i = 0; i < 16; ++i)
+        s[b][i] = mie::extend::holds(seen, b * 32 + in_block(i, 0)) ? s[b][i] : -INFINITY;
   }
 #pragma unroll
   for (int b = 0; b < L::NB; ++b)
@@ -333,10 +354,13 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile
   w.row_head = kvh * a.group.d + row - token * a.group.d;
   w.position = base + token;
   w.slope = a.slopes ? a.slopes[w.row_head] * kLog2e : 0.f;
-  w.p_first = base + static_cast<int>(a.group.div(min(row0, p.rows - 1)));
-  w.p_last = base + static_cast<int>(a.group.div(min(row0 + 32, p.rows) - 1));
-  w.high = row0 < p.rows ? min(end, max(w.p_last + 1, p.prefix)) : first;
-  w.low = a.window > 0 ? max(0, w.p_first - a.window + 1) : 0;
+  const int p_first = base + static_cast<int>(a.group.div(min(row0, p.rows - 1)));
+  const int p_last = base + static_cast<int>(a.group.div(min(row0 + 32, p.rows) - 1));
+  w.keys = mie::extend::keys_of(a, p, w.position);
+  w.shared = mie::extend::shared_keys(a, p, p_first, p_last);
+  w.some = mie::extend::Range{mie::extend::keys_of(a, p, p_first).low,
+                              row0 < p.rows ? mie::extend::keys_of(a, p, p_last).high : 0};
+  const mie::extend::Range shared = mie::extend::shared_keys(a, p, p.p_first, p.p_last);  // by every row of the tile
   const char* qp = a.q + (p.start + token) * a.q_st + w.row_head * a.q_sh + h * 16;
 #pragma unroll
   for (int c = 0; c < L::NQ; ++c) w.q[c] = *reinterpret_cast<const u32x4*>(qp + c * 32);
@@ -347,41 +371,68 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile
 #pragma unroll
     for (int i = 0; i < 16; ++i) w.o[n][i] = 0.f;
 
-  // Loading: lane's n-th 16-byte piece of a tile is at byte ((4 n + wave) 64 +
-  // lane) 16 of the LDS buffer, so in key `key[n]`'s row.
+  // Loading.  A wave brings kKeys consecutive keys of a tile, the lane's n-th
+  // 16-byte piece to byte ((wave kLoads + n) 64 + lane) 16 of the LDS buffer.
   const char* k_head = a.k_pool + kvh * a.shead;
   const char* v_head = a.v_pool + kvh * a.shead;
-  int key[L::kLoads], k_piece[L::kLoads], v_piece[L::kLoads];
+  const int32_t* table = a.tables + p.b * a.table_stride;
+  int in_wave[L::kLoads], k_piece[L::kLoads], v_piece[L::kLoads];  // the piece's key and its bytes in that key's row
 #pragma unroll
   for (int n = 0; n < L::kLoads; ++n) {
-    const int at = (n * 4 + wave) * 64 + lane;
-    key[n] = at / L::CH;
-    k_piece[n] = ((at - key[n] * L::CH) ^ key_swizzle<L::CH>(key[n])) * 16;
-    v_piece[n] = ((at - key[n] * L::CH) ^ value_swizzle<T, L::CH>(key[n])) * 16;
+    const int at = n * 64 + lane;
+    in_wave[n] = at / L::CH;
+    k_piece[n] = ((at - in_wave[n] * L::CH) ^ key_swizzle<L::CH>(wave * L::kKeys + in_wave[n])) * 16;
+    v_piece[n] = ((at - in_wave[n] * L::CH) ^ value_swizzle<T, L::CH>(wave * L::kKeys + in_wave[n])) * 16;
   }
+  auto to_lds = [&](const char* from, char* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+  };
   // Table entries are loaded a tile ahead and looked at when they are used:
-  // waiting for one is waiting for every load before it.
-  const int32_t* table = a.tables + p.b * a.table_stride;
+  // waiting for one is waiting for every load before it.  Where blocks hold
+  // whole multiples of kKeys the wave's keys are one block's, and its address
+  // is the wave's; keys past the end are places behind the last one's in its
+  // block.  Otherwise every lane finds its own, the last key again past the end.
   int32_t id[L::kLoads];
+  auto group_of = [&](int k0) { return min(k0 + wave * L::kKeys, (end - 1) & -L::kKeys); };
   auto look_up = [&](int k0) {
+    if (a.whole_blocks) {
+      id[0] = table[min(static_cast<int>(a.bs.div(group_of(k0))), a.table_width - 1)];
+    } else {
 #pragma unroll
-    for (int n = 0; n < L::kLoads; ++n)
-      id[n] = table[min(static_cast<int>(a.bs.div(min(k0 + key[n], end - 1))), a.table_width - 1)];
+      for (int n = 0; n < L::kLoads; ++n)
+        id[n] = table[min(static_cast<int>(a.bs.div(min(k0 + wave * L::kKeys + in_wave[n], end - 1))), a.table_width - 1)];
+    }
   };
   auto load = [&](int k0, char* k_tile, char* v_tile) {
+    k_tile += wave * L::kLoads * 1024;
+    v_tile += wave * L::kLoads * 1024;
+    if (a.whole_blocks) {
+      const int key = group_of(k0);
+      const int blk = a.bs.div(key);
+      const int32_t block = __builtin_amdgcn_readfirstlane(id[0]);
+      const bool bad = static_cast<uint32_t>(block) >= static_cast<uint32_t>(a.num_blocks) || blk >= a.table_width;
+      const int64_t off =
+          (bad ? 0 : block) * a.sblk + static_cast<int64_t>(key - blk * static_cast<int>(a.bs.d)) * L::kRowBytes;
+#pragma unroll
+      for (int n = 0; n < L::kLoads; ++n) {
+        to_lds(k_head + off + static_cast<uint32_t>(in_wave[n] * L::kRowBytes + k_piece[n]), k_tile + n * 1024);
+        to_lds(v_head + off + static_cast<uint32_t>(in_wave[n] * L::kRowBytes + v_piece[n]), v_tile + n * 1024);
+      }
+      if (bad) s_bad = 1;
+      return;
+    }
     bool any = false;
 #pragma unroll
     for (int n = 0; n < L::kLoads; ++n) {
-      const int at_key = min(k0 + key[n], end - 1);
-      const int blk = a.bs.div(at_key);
+      const int key = min(k0 + wave * L::kKeys + in_wave[n], end - 1);
+      const int blk = a.bs.div(key);
       const bool bad = static_cast<uint32_t>(id[n]) >= static_cast<uint32_t>(a.num_blocks) || blk >= a.table_width;
-      const int64_t off = (bad ? 0 : id[n]) * a.sblk + (at_key - blk * static_cast<int>(a.bs.d)) * L::kRowBytes;
+      const int64_t off =
+          (bad ? 0 : id[n]) * a.sblk + static_cast<int64_t>(key - blk * static_cast<int>(a.bs.d)) * L::kRowBytes;
       any |= bad;
-      const int to = (n * 4 + wave) * 1024;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(k_head + off + k_piece[n]),
-                                       (__attribute__((address_space(3))) void*)(k_tile + to), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(v_head + off + v_piece[n]),
-                                       (__attribute__((address_space(3))) void*)(v_tile + to), 16, 0, 0);
+      to_lds(k_head + off + k_piece[n], k_tile + n * 1024);
+      to_lds(v_head + off + v_piece[n], v_tile + n * 1024);
     }
     if (__any(any)) s_bad = 1;
   };
@@ -400,7 +451,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile
   }
   auto step = [&](char* k_here, char* v_here, char* k_next, char* v_next) {
     arrive();
-    if (!mie::extend::all_see(a, p, k0, k0 + L::KT)) {
+    if (!mie::extend::holds(shared, k0, k0 + L::KT)) {
       if (drop_not_finite<T, D>(v_here, wave)) s_odd = 1;
       __syncthreads();
     }
@@ -408,7 +459,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile
       load(k0 + L::KT, k_next, v_next);
       if (k0 + 2 * L::KT < end) look_up(k0 + 2 * L::KT);
     }
-    if (k0 < w.high && k0 + L::KT > w.low) attend<T, D>(a, p, w, at, k_here, v_here, k0);
+    if (k0 < w.some.high && k0 + L::KT > w.some.low) attend<T, D>(a, w, at, k_here, v_here, k0);
     k0 += L::KT;
   };
   while (k0 < end) {
