@@ -378,11 +378,35 @@ struct Plan {
   int64_t bytes;
 };
 
+// Tiles of 128 rows read K and V an eighth as often as those of 16, but take
+// a wave per 32 rows and stage through LDS: they pay from some work on, and
+// where a sequence has more rows than the small ones hold.  The work is
+// tokens x heads x keys x head_dim, the keys those of a middle token.
+// Measured on MI355X, us with 16 / 128 rows (new tokens per sequence + those
+// before), the work in millions behind it:
+//   bfloat16, 12 heads x 64: 1 x 16 + 2000 (25) 12.9 / 14.0; 1 x 256 + 0 (25)
+//   8.6 / 10.9; 8 x 16 + 1000 (99) 14.6 / 14.3; 1 x 64 + 4000 (198) 21.9 /
+//   18.7; 1 x 1000 + 0 (384) 25.2 / 19.6; 8 x 256 + 1000 (1774) 60.7 / 35.6.
+//   32 heads over 8 x 128: 1 x 16 + 2000 (132) 17.0 / 18.1; 1 x 256 + 0 (134)
+//   13.1 / 14.2; 8 x 16 + 1000 (528) 33.8 / 23.8; 1 x 256 + 4000 (4328) 119 / 56.
+//   float32, 12 x 64: 1 x 1000 + 0 (384) 39.9 / 50.3; 8 x 64 + 1000 (406) 42 /
+//   47; 1 x 256 + 4000 (812) 75 / 60; 8 x 256 + 1000 (1774) 121 / 102.  32 over
+//   8 x 128: 1 x 256 + 0 (134) 25 / 43; 8 x 16 + 1000 (528) 66 / 51; 1 x 1000
+//   + 0 (2048) 193 / 137; 64 x 4 + 2000 (2099, 16 rows) 214 / 566.
+bool many_rows(int64_t tokens, int max_new, int64_t keys, int group, int kv_heads, int head_dim, int dtype) {
+  const int64_t work = tokens * group * kv_heads * (keys - std::min<int64_t>(max_new, keys) / 2) * head_dim;
+  if (dtype == MIE_DTYPE_F32) return static_cast<int64_t>(max_new) * group >= 64 && work >= 500'000'000;
+  return static_cast<int64_t>(max_new) * group > kFewRows && work >= 160'000'000;
+}
+
 // Row tiles: as many as the batch can have (the lengths are on the device).
 // The keys are split until the tiles make kGroupsWanted workgroups.
-Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int group, int kv_heads, int head_dim) {
+Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int group, int kv_heads, int head_dim,
+               int dtype) {
   Plan p;
-  const int rows = p.rows = static_cast<int64_t>(max_new) * group >= 64 ? kTileRows : kFewRows;
+  const int64_t keys = window > 0 ? std::min(max_len, window) : max_len;
+  const int rows = p.rows =
+      many_rows(tokens, max_new, keys, group, kv_heads, head_dim, dtype) ? kTileRows : kFewRows;
   const int64_t most = (static_cast<int64_t>(max_new) * group + rows - 1) / rows;
   p.tiles = static_cast<int64_t>(max_new) * group <= rows
                 ? batch
@@ -456,7 +480,7 @@ extern "C" int64_t mie_paged_extend_workspace(int32_t tokens, int32_t batch, int
     return -rc;
   if (tokens == 0 || max_new == 0) return 0;
   return make_plan(tokens, batch, std::min(max_new, tokens), max_context_len, window, num_heads / num_kv_heads,
-                   num_kv_heads, head_dim)
+                   num_kv_heads, head_dim, dtype)
       .bytes;
 }
 
@@ -492,7 +516,7 @@ extern "C" int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q
     return mie::fail(MIE_ERR_INVALID, "%s: rows of q, out and the pools must be 16-byte aligned", what);
   max_new = std::min(max_new, tokens);
   const int group = num_heads / num_kv_heads;
-  const Plan plan = make_plan(tokens, batch, max_new, max_context_len, window, group, num_kv_heads, head_dim);
+  const Plan plan = make_plan(tokens, batch, max_new, max_context_len, window, group, num_kv_heads, head_dim, dtype);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return mie::fail(MIE_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", what,
                      static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));

@@ -110,7 +110,7 @@ struct Tile {
   static constexpr int kLoads = kBytes / 4096;  // 16-byte loads per lane for K, and as many for V
   static constexpr int kKeys = KT / 4;          // keys a wave loads
   static constexpr int NQ = D / Products<T>::kDims, NB = KT / 32, ND = D / 32;
-  static_assert(kBytes % 4096 == 0 && 16 % kKeys == 0, "a tile divides among four waves");
+  static_assert(kBytes % 4096 == 0 && 16 % kKeys == 0, "a tile divides among the waves");
 };
 
 // Where a lane reads in a tile.  XORs touch the bits below a row only, so an
@@ -207,7 +207,7 @@ __device__ __forceinline__ void multiply_values(State<T, D>& w, const Reads<T, D
   }
 }
 
-// Replaces this wave's quarter of a tile's values that are not finite by 0;
+// Replaces this wave's share of a tile's values that are not finite by 0;
 // whether there were any.
 template <typename T, int D>
 __device__ __forceinline__ bool drop_not_finite(char* tile, int wave) {
@@ -269,8 +269,9 @@ __device__ __forceinline__ void attend(const Args& a, State<T, D>& w, const Read
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
 #pragma unroll
-    for (int c = 0; c < L::NQ; ++c)
+    for (int c = 0; c < L::NQ; ++c) {
       s[b] = Products<T>::scores(*reinterpret_cast<const u32x4*>(k_tile + at.key(b, c)), w.q[c], s[b]);
+    }
   }
   float top = -INFINITY, scale = a.scale;  // a positive scale goes into the exponential's operand
   const int key0 = fresh(k0 + 4 * ((threadIdx.x & 63) >> 5));
@@ -324,8 +325,8 @@ __device__ __forceinline__ void attend(const Args& a, State<T, D>& w, const Read
 }
 
 // grid = tiles x parts x kv_heads, the K/V head fastest, a sequence's last
-// tiles (the longest) first.
-template <typename T, int D>
+// tiles (the longest) first.  WHOLE: blocks hold a multiple of 16 keys.
+template <typename T, int D, bool WHOLE>
 __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile_kernel(Args a) {
   using L = Tile<T, D>;
   __shared__ __align__(16) char s_k0[L::kBytes];
@@ -393,48 +394,43 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile
   // whole multiples of kKeys the wave's keys are one block's, and its address
   // is the wave's; keys past the end are places behind the last one's in its
   // block.  Otherwise every lane finds its own, the last key again past the end.
-  int32_t id[L::kLoads];
+  int32_t id[WHOLE ? 1 : L::kLoads];
   auto group_of = [&](int k0) { return min(k0 + wave * L::kKeys, (end - 1) & -L::kKeys); };
+  auto key_of = [&](int k0, int n) { return min(k0 + wave * L::kKeys + in_wave[n], end - 1); };
   auto look_up = [&](int k0) {
-    if (a.whole_blocks) {
+    if constexpr (WHOLE) {
       id[0] = table[min(static_cast<int>(a.bs.div(group_of(k0))), a.table_width - 1)];
     } else {
 #pragma unroll
       for (int n = 0; n < L::kLoads; ++n)
-        id[n] = table[min(static_cast<int>(a.bs.div(min(k0 + wave * L::kKeys + in_wave[n], end - 1))), a.table_width - 1)];
+        id[n] = table[min(static_cast<int>(a.bs.div(key_of(k0, n))), a.table_width - 1)];
     }
   };
-  auto load = [&](int k0, char* k_tile, char* v_tile) {
-    k_tile += wave * L::kLoads * 1024;
-    v_tile += wave * L::kLoads * 1024;
-    if (a.whole_blocks) {
-      const int key = group_of(k0);
-      const int blk = a.bs.div(key);
-      const int32_t block = __builtin_amdgcn_readfirstlane(id[0]);
-      const bool bad = static_cast<uint32_t>(block) >= static_cast<uint32_t>(a.num_blocks) || blk >= a.table_width;
-      const int64_t off =
-          (bad ? 0 : block) * a.sblk + static_cast<int64_t>(key - blk * static_cast<int>(a.bs.d)) * L::kRowBytes;
-#pragma unroll
-      for (int n = 0; n < L::kLoads; ++n) {
-        to_lds(k_head + off + static_cast<uint32_t>(in_wave[n] * L::kRowBytes + k_piece[n]), k_tile + n * 1024);
-        to_lds(v_head + off + static_cast<uint32_t>(in_wave[n] * L::kRowBytes + v_piece[n]), v_tile + n * 1024);
-      }
+  auto row_of = [&](int key, int32_t block, bool& bad) {
+    const int blk = a.bs.div(key);
+    bad = static_cast<uint32_t>(block) >= static_cast<uint32_t>(a.num_blocks) || blk >= a.table_width;
+    return (bad ? 0 : block) * a.sblk + static_cast<int64_t>(key - blk * static_cast<int>(a.bs.d)) * L::kRowBytes;
+  };
+  int64_t next_off = 0;  // WHOLE: the next tile's row of this wave
+  auto aim = [&](int k0) {
+    if constexpr (WHOLE) {
+      bool bad;
+      next_off = row_of(group_of(k0), __builtin_amdgcn_readfirstlane(id[0]), bad);
       if (bad) s_bad = 1;
-      return;
     }
-    bool any = false;
-#pragma unroll
-    for (int n = 0; n < L::kLoads; ++n) {
-      const int key = min(k0 + wave * L::kKeys + in_wave[n], end - 1);
-      const int blk = a.bs.div(key);
-      const bool bad = static_cast<uint32_t>(id[n]) >= static_cast<uint32_t>(a.num_blocks) || blk >= a.table_width;
-      const int64_t off =
-          (bad ? 0 : id[n]) * a.sblk + static_cast<int64_t>(key - blk * static_cast<int>(a.bs.d)) * L::kRowBytes;
-      any |= bad;
-      to_lds(k_head + off + k_piece[n], k_tile + n * 1024);
-      to_lds(v_head + off + v_piece[n], v_tile + n * 1024);
+  };
+  auto bring = [&](int k0, int n, char* k_tile, char* v_tile) {
+    const int to = (wave * L::kLoads + n) * 1024;
+    if constexpr (WHOLE) {
+      to_lds(k_head + next_off + static_cast<uint32_t>(in_wave[n] * L::kRowBytes + k_piece[n]), k_tile + to);
+      to_lds(v_head + next_off + static_cast<uint32_t>(in_wave[n] * L::kRowBytes + v_piece[n]), v_tile + to);
+    } else {
+      bool bad;
+      const int64_t off = row_of(key_of(k0, n), id[n], bad);
+      to_lds(k_head + off + k_piece[n], k_tile + to);
+      to_lds(v_head + off + v_piece[n], v_tile + to);
+      if (__any(bad)) s_bad = 1;
     }
-    if (__any(any)) s_bad = 1;
   };
   // Everything this wave has loaded is in LDS, and every wave's is after the barrier.
   auto arrive = [&]() {
@@ -446,8 +442,10 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile
   int k0 = first;
   if (k0 < end) {
     look_up(k0);
-    load(k0, s_k0, s_v0);
-    if (k0 + L::KT < end) look_up(k0 + L::KT);
+    aim(k0);
+#pragma unroll
+    for (int n = 0; n < L::kLoads; ++n) bring(k0, n, s_k0, s_v0);
+    look_up(k0 + L::KT);
   }
   auto step = [&](char* k_here, char* v_here, char* k_next, char* v_next) {
     arrive();
@@ -455,9 +453,12 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile
       if (drop_not_finite<T, D>(v_here, wave)) s_odd = 1;
       __syncthreads();
     }
+    // (Past the last tile its last keys come again, and nobody reads them.)
     if (k0 + L::KT < end) {
-      load(k0 + L::KT, k_next, v_next);
-      if (k0 + 2 * L::KT < end) look_up(k0 + 2 * L::KT);
+      aim(k0 + L::KT);
+#pragma unroll
+      for (int n = 0; n < L::kLoads; ++n) bring(k0 + L::KT, n, k_next, v_next);
+      look_up(k0 + 2 * L::KT);
     }
     if (k0 < w.some.high && k0 + L::KT > w.some.low) attend<T, D>(a, w, at, k_here, v_here, k0);
     k0 += L::KT;
@@ -473,7 +474,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile
 #pragma unroll
   for (int n = 0; n < L::ND * 4; ++n)
     o[n] = f32x4{w.o[n / 4][n % 4 * 4], w.o[n / 4][n % 4 * 4 + 1], w.o[n / 4][n % 4 * 4 + 2], w.o[n / 4][n % 4 * 4 + 3]};
-  __syncthreads();
+  arrive();
   if (s_bad | s_odd) {
     f32x4 mended[L::ND * 4];
     float mended_sum = sum;
@@ -503,14 +504,22 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile
   }
 }
 
+template <typename T, int D>
+void launch_tile(const Args& a, uint32_t groups, hipStream_t st) {
+  if (a.whole_blocks)
+    extend_tile_kernel<T, D, true><<<groups, 256, 0, st>>>(a);
+  else
+    extend_tile_kernel<T, D, false><<<groups, 256, 0, st>>>(a);
+}
+
 template <typename T>
 void launch_dim(const Args& a, int head_dim, uint32_t groups, hipStream_t st) {
   switch (head_dim) {
-    case 32: extend_tile_kernel<T, 32><<<groups, 256, 0, st>>>(a); break;
-    case 64: extend_tile_kernel<T, 64><<<groups, 256, 0, st>>>(a); break;
-    case 96: extend_tile_kernel<T, 96><<<groups, 256, 0, st>>>(a); break;
-    case 128: extend_tile_kernel<T, 128><<<groups, 256, 0, st>>>(a); break;
-    default: extend_tile_kernel<T, 256><<<groups, 256, 0, st>>>(a); break;
+    case 32: launch_tile<T, 32>(a, groups, st); break;
+    case 64: launch_tile<T, 64>(a, groups, st); break;
+    case 96: launch_tile<T, 96>(a, groups, st); break;
+    case 128: launch_tile<T, 128>(a, groups, st); break;
+    default: launch_tile<T, 256>(a, groups, st); break;
   }
 }
 

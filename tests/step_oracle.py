@@ -81,29 +81,28 @@ def extend(q, k, v, length, *, scale, softcap=0.0, slopes=None, window=0, prefix
     n, heads, dim = q.shape
     group = heads // k.shape[1]
     out, bound = torch.zeros_like(q), torch.zeros_like(q)
-    j = torch.arange(length)
-    for i in range(n):
-        p = length - n + i
-        ok = (j <= p) | (j < prefix)
-        if window:
-            ok &= j > p - window
-        ok = ok.nonzero()[:, 0]
-        if p < 0 and prefix == 0 or len(ok) == 0:
-            continue
-        for h in range(heads):
-            kk, vv = k[ok, h // group], v[ok, h // group]
-            s = kk @ q[i, h] * scale
-            d = (dim + 4) * eps_dot * (kk.abs() @ q[i, h].abs()) * abs(scale)
-            if softcap:
-                s = softcap * torch.tanh(s / softcap)
-                d = d + softcap * eps_tanh
-            if slopes is not None:
-                far = float(slopes[h]) * (p - ok).abs().double()
-                s = s - far
-                d = d + 3 * eps_dot * far
-            d = d + 4 * eps_dot * s.abs()
-            w = torch.softmax(s, dim=0)
-            out[i, h] = w @ vv
-            rel = 4 * d.max() + 2.0**-21 + eps_p + (len(ok) + 16) * 2.0**-24
-            bound[i, h] = rel * (w @ vv.abs())
+    if n == 0 or length == 0:
+        return out, bound
+    j, p = torch.arange(length)[None], torch.arange(length - n, length)[:, None]
+    ok = (j <= p) | (j < prefix)
+    if window:
+        ok &= j > p - window
+    seen = ok.sum(-1, keepdim=True)
+    for h in range(heads):
+        kk, vv = k[:, h // group], v[:, h // group]
+        s = q[:, h] @ kk.T * scale
+        d = (dim + 4) * eps_dot * (q[:, h].abs() @ kk.abs().T) * abs(scale)
+        if softcap:
+            s = softcap * torch.tanh(s / softcap)
+            d = d + softcap * eps_tanh
+        if slopes is not None:
+            far = float(slopes[h]) * (p - j).abs().double()
+            s = s - far
+            d = d + 3 * eps_dot * far
+        d = torch.where(ok, d + 4 * eps_dot * s.abs(), 0.0)
+        w = torch.softmax(s.masked_fill(~ok, float("-inf")), dim=-1)
+        w = torch.where(seen > 0, w, 0.0)
+        out[:, h] = w @ vv
+        rel = 4 * d.amax(-1, keepdim=True) + 2.0**-21 + eps_p + (seen + 16) * 2.0**-24
+        bound[:, h] = rel * (w @ vv.abs())
     return out, bound

@@ -196,6 +196,109 @@ def test_scores_of_the_lowest_value(dtype):
     assert float((got[:3].double().cpu() - want).abs().max()) < float(bound) + 2.0**-8
 
 
+# Enough rows and keys for the tiles of 128 rows (the tests above stay below them).
+MANY = dict(new=[300, 1, 70, 0, 33], old=[500, 700, 0, 60, 95], heads=32, kv_heads=4)
+
+
+@pytest.mark.parametrize("dim,block_size", [(32, 16), (64, 16), (64, 7), (64, 32), (96, 16), (96, 24), (128, 16),
+                                            (128, 1), (256, 16), (256, 40)])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_many_rows(dim, block_size, dtype):
+    print_case("extend many rows", dim, block_size, dtype)
+    scale = 64 // dim or 1
+    c = batch(MANY["new"], MANY["old"], 32 * scale, 4 * scale, dim, block_size, dtype, seed=dim, extra=1, pad=2)
+    check(c, call(c))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(24, 24), (40, 8), (66, 2)])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_many_rows_of_other_groups(heads, kv_heads, dtype):
+    print_case("extend many rows", heads, kv_heads, dtype)
+    c = batch(MANY["new"], MANY["old"], heads, kv_heads, 64, 16, dtype, seed=heads)
+    check(c, call(c))
+
+
+@pytest.mark.parametrize("option", OPTIONS, ids=str)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_scores_and_masks_of_many_rows(option, dtype):
+    print_case("extend many rows option", option, dtype)
+    new, old = [290, 1, 101], [700, 400, 200]
+    # A window bounds the work that is counted: more heads for it.
+    heads = 32 if option.get("window", 10**6) > 500 else 256
+    c = batch(new, old, heads, 4, 64, 16, dtype, seed=7)
+    kw, want = dict(option), dict(option)
+    if "slopes" in option:
+        want["slopes"] = 2.0 ** -(torch.arange(heads).double() % 7 * 1.5)
+        kw["slopes"] = want["slopes"].float().to(DEV)
+    if "prefix" in option:
+        kw["prefix_lens"] = torch.tensor(kw.pop("prefix"), dtype=torch.int32, device=DEV)
+        want["prefix"] = [min(p, n) for p, n in zip(option["prefix"], c["len_list"])]
+    check(c, call(c, **kw), **want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_many_rows_over_a_split_context(dtype):
+    print_case("extend many rows split", dtype)
+    c = batch([150, 40], [6000, 2500], 8, 1, 64, 16, dtype, seed=3, heavy=0.01)
+    check(c, call(c))
+    check(c, call(c, window=3000), window=3000)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("window", [0, 500])
+def test_what_many_rows_do_not_see_has_no_part_in_them(dtype, window):
+    print_case("extend many rows masked nan", dtype, window)
+    for poison in (float("nan"), float("inf"), -float("inf")):
+        for where in ("k", "v"):
+            for block_size in (16, 5):
+                c = batch([400], [500], 32, 4, 64, block_size, dtype, seed=4)
+                clean = call(c, window=window)
+                at = 700
+                c[where][1, c["tables"][0, at // block_size].item(), :, at % block_size, 5] = poison
+                got = call(c, window=window)
+                rows = torch.arange(500, 900)
+                sees = ((rows >= at) & (rows < at + (window or 10**6))).to(DEV)
+                assert torch.equal(got[~sees], clean[~sees]), (poison, where)
+                if where == "v":
+                    assert not bool(got[sees][:, :, 5].isfinite().any())
+                    if poison == poison:
+                        assert bool((got[sees][:, :, 5] == poison).all())
+                    others = torch.arange(64, device=DEV) != 5
+                    assert bool(got[sees][:, :, others].isfinite().all())
+                elif poison != poison:
+                    assert bool(got[sees].isnan().all())
+
+
+def test_many_rows_with_lengths_and_tables_out_of_bounds():
+    print_case("extend many rows bad tables")
+    for dtype in (F32, BF16):
+        for block_size in (16, 9):
+            c = batch([200, 300, 100, 40], [400, 400, 600, 0], 32, 4, 64, block_size, dtype, seed=6)
+            c["tables"][1, 450 // block_size] = -1         # rows from its first token on see it
+            c["tables"][2, 100 // block_size] = 2**31 - 1  # every row does
+            c["lens"][3] = 10000                           # past the bound, and its table row
+            got = call(c)
+            check(c, got, skip=(1, 2, 3))
+            first = 450 // block_size * block_size - 400
+            assert bool(got[200 + first : 500].isnan().all()) and bool(got[500:640].isnan().all())
+            assert bool(got[200 : 200 + first].isfinite().all())
+            # A bad entry no token sees: behind the window.
+            c = batch([300], [900], 128, 4, 64, block_size, dtype, seed=6)
+            c["tables"][0, 2] = -1
+            check(c, call(c, window=600), window=600)
+
+
+def test_many_rows_with_broken_starts():
+    print_case("extend many rows bad starts")
+    c = batch([200, 300, 100], [400, 500, 300], 32, 4, 64, 16, BF16, seed=6)
+    c["starts"][:] = torch.tensor([0, -5, 10000, 3])
+    call(c, max_new=400, max_len=900)
+    c["lens"][:] = torch.tensor([-4, 0, 1])
+    c["starts"][:] = torch.tensor([0, 200, 500, 600])
+    got = call(c, max_new=300, max_len=900)
+    assert bool((got[:599] == 0).all()) and bool(got[599].isfinite().all())
+
+
 def test_lengths_and_tables_out_of_bounds():
     print_case("extend bad tables")
     for dtype in (F32, BF16):
@@ -312,5 +415,8 @@ def test_two_captured_steps_and_streams_keep_apart():
 
 def test_the_same_call_gives_the_same_bits():
     print_case("extend twice")
-    c = batch([1, 300, 5], [5000, 100, 900], 6, 2, 128, 16, BF16, seed=12)
-    assert torch.equal(call(c), call(c))
+    for dtype in (F32, BF16):
+        c = batch([1, 300, 5], [5000, 100, 900], 6, 2, 128, 16, dtype, seed=12)
+        assert torch.equal(call(c), call(c))
+        c = batch([1, 3, 5], [500, 100, 900], 6, 2, 128, 16, dtype, seed=12)
+        assert torch.equal(call(c), call(c))
