@@ -13,12 +13,13 @@
 //
 // Alternatives.  A row's `top` best keys (value, then the lower index) are
 // found in the same pass.  A wave keeps a bound that at least `top` of its
-// values so far reach - at first the top-th largest of its lanes' maxima over
-// the first chunk, 64 lanes x 32 values - and writes the few values above it
-// to a list in LDS; a list that fills up is cut to its `top` best, which raises
-// the bound.  A wave's values come in the order of their indices, so a later
-// one equal to the bound is never among the best.  In the end the lists of
-// the four waves are ranked by counting.
+// values so far reach: what the top-th largest of its lanes' maxima is, found
+// bit by bit with ballots and left at 16 bits, from the first chunk (64 lanes
+// x 16 values) and again after the 2nd, 4th, 8th, ...  The few values above it
+// go to a list in LDS; a list that fills up is cut to its `top` best, which
+// raises the bound too.  A wave's values come in the order of their indices,
+// so one equal to a bound that earlier values set is never among the best.  In
+// the end the lists of the four waves are ranked by counting.
 //
 // A row with a NaN or +inf has no finite result: only the order of its
 // alternatives is left, which is found by one pass for each.
@@ -116,36 +117,44 @@ struct List {
   float bound;
 };
 
-// The k-th largest of the lanes' values (k <= 64).
-__device__ __forceinline__ float kth_of_lanes(float x, int k) {
-  float last = -INFINITY;
-  bool in = true;
-  for (int j = 0; j < k; ++j) {
-    last = mie::wave_max(in ? x : -INFINITY);
-    const uint64_t equal = __ballot(in && x == last);
-    if (equal == 0) break;  // nothing above -inf is left
-    if ((threadIdx.x & 63) == __builtin_ctzll(equal)) in = false;
+// A value that at least k of the lanes' reach (k <= 64): the k-th largest,
+// down to 16 bits of its rank.
+__device__ __forceinline__ float reached_by(float x, int k) {
+  const uint32_t u = __float_as_uint(x);
+  const uint32_t rank = u & 0x80000000u ? ~u : u | 0x80000000u;
+  uint32_t bound = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t higher = bound | 1u << bit;
+    if (__popcll(__ballot(rank >= higher)) >= k) bound = higher;
   }
-  return last;
+  // Below the smallest rank of a number every value reaches -inf.
+  return bound < 0x00800000u ? -INFINITY : __uint_as_float(bound & 0x80000000u ? bound & 0x7fffffffu : ~bound);
 }
 
-// Cuts the list to its `top` best, best first.
-__device__ __attribute__((noinline)) void cut(List& list, int top) {
+// Cuts `count` keys to the `top` best, best first; the last one's value, or
+// -inf where there are fewer.  Apart from the kernels, whose registers it
+// would take: everything goes in and out by value.
+__device__ __attribute__((noinline)) float best_of(__attribute__((address_space(3))) uint64_t* keys, int count,
+                                                   int top) {
   const int lane = threadIdx.x & 63;
   uint64_t mine[kCap / 64];
 #pragma unroll
-  for (int j = 0; j < kCap / 64; ++j) mine[j] = j * 64 + lane < list.count ? list.keys[j * 64 + lane] : 0;
-  const int kept = min(list.count, top);
+  for (int j = 0; j < kCap / 64; ++j) mine[j] = j * 64 + lane < count ? keys[j * 64 + lane] : 0;
   uint64_t last = ~0ull;
-  for (int k = 0; k < kept; ++k) {
+  for (int k = 0; k < min(count, top); ++k) {
     uint64_t best = 0;
 #pragma unroll
     for (int j = 0; j < kCap / 64; ++j) best = mine[j] < last && mine[j] > best ? mine[j] : best;
     last = wave_max(best);
-    if (lane == 0) list.keys[k] = last;
+    if (lane == 0) keys[k] = last;
   }
-  list.count = kept;
-  if (kept == top) list.bound = value_of(last);
+  return count < top ? -INFINITY : value_of(last);
+}
+__device__ __forceinline__ void cut(List& list, int top) {
+  const float bound = best_of((__attribute__((address_space(3))) uint64_t*)list.keys, list.count, top);
+  list.count = __builtin_amdgcn_readfirstlane(min(list.count, top));
+  list.bound = fmaxf(list.bound, bound);
 }
 
 // Adds the lanes' keys for which `want` holds; there is room.
@@ -159,13 +168,13 @@ __device__ __forceinline__ void push(List& list, float x, int index, bool want) 
 
 template <typename T> struct Chunk;
 template <> struct Chunk<float> {
-  static constexpr int VEC = 4, U = 8;
+  static constexpr int VEC = 4, U = 4;
   u32x4 v[U];
   __device__ __forceinline__ float get(int u, int j) const { return __uint_as_float(v[u][j]); }
   static constexpr uint32_t kLowest = 0xff800000u;  // -inf
 };
 template <> struct Chunk<uint16_t> {
-  static constexpr int VEC = 8, U = 4;
+  static constexpr int VEC = 8, U = 2;
   u32x4 v[U];
   __device__ __forceinline__ float get(int u, int j) const {
     return j % 2 ? mie::bf16_hi(v[u][j / 2]) : mie::bf16_lo(v[u][j / 2]);
@@ -195,7 +204,8 @@ __device__ __forceinline__ void finish(const LogprobsArgs& a, int64_t row, Sums 
 
 // A row without finite results: NaN, and the alternatives one after the other.
 template <typename T>
-__device__ __attribute__((noinline)) void finish_not_finite(const LogprobsArgs& a, int64_t row, uint64_t* s_best) {
+__device__ __attribute__((noinline)) void finish_not_finite(LogprobsArgs a, int64_t row) {
+  __shared__ uint64_t s_best[kWaves];
   const T* x = reinterpret_cast<const T*>(a.logits) + row * a.stride;
   if (threadIdx.x == 0) {
     if (a.logprobs) a.logprobs[row] = NAN;
@@ -237,7 +247,6 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(LogprobsArg
   using C = Chunk<T>;
   constexpr int VEC = C::VEC, U = C::U;
   __shared__ uint64_t s_keys[TOP ? kWaves * kCap : 1];
-  __shared__ uint64_t s_best[kWaves];
   __shared__ int s_count[kWaves];
   const int64_t row = static_cast<int>(blockIdx.x) / a.slices;
   const int slice = static_cast<int>(blockIdx.x) % a.slices;
@@ -284,15 +293,25 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(LogprobsArg
   };
   if (slice == 0 && wave == 0 && head > 0) edge(0, head);
 
-  for (int c = first; c < last; c += U * kThreads) {
-    C chunk;
+  auto load = [&](C& chunk, int c) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = c + u * kThreads + threadIdx.x;
-      if (i < last)
-        chunk.v[u] = __builtin_nontemporal_load(xv + i);
-      else
-        chunk.v[u] = u32x4{C::kLowest, C::kLowest, C::kLowest, C::kLowest};
+      chunk.v[u] = __builtin_nontemporal_load(xv + min(i, last - 1));
+    }
+  };
+  C chunk, next;
+  float lane_most = -INFINITY;
+  if (first < last) load(chunk, first);
+  for (int c = first, n = 1; c < last; c += U * kThreads, ++n, chunk = next) {
+    load(next, c + U * kThreads);
+    // What was loaded past the end counts as -inf; looked at here, where the
+    // loads of the next chunk are under way.
+    if (c + U * kThreads > last) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c + u * kThreads + static_cast<int>(threadIdx.x) >= last)
+          chunk.v[u] = u32x4{C::kLowest, C::kLowest, C::kLowest, C::kLowest};
     }
     float top[U];
 #pragma unroll
@@ -310,17 +329,18 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(LogprobsArg
 #pragma unroll
       for (int j = 0; j < VEC; ++j) add(chunk.get(u, j), j % 4);
     if constexpr (TOP) {
-      // In the first chunk values equal to the bound are taken too.
-      const bool start = c == first;
-      if (start) list.bound = kth_of_lanes(most, a.top);
+      // Values equal to the bound are taken where this chunk raised it.
+      bool start = c == first;
+      lane_most = fmaxf(lane_most, most);
+      if ((n & (n - 1)) == 0) {
+        const float bound = reached_by(lane_most, a.top);
+        start |= bound > list.bound;
+        list.bound = fmaxf(list.bound, bound);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (!__any(start ? top[u] >= list.bound : top[u] > list.bound)) continue;
-        if (list.count + 64 * VEC > kCap) {
-          const float bound = list.bound;
-          cut(list, a.top);
-          list.bound = fmaxf(list.bound, bound);
-        }
+        if (list.count + 64 * VEC > kCap) cut(list, a.top);
         const int i = c + u * kThreads + threadIdx.x;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -363,7 +383,7 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(LogprobsArg
   }
   if (a.slices == 1) {
     if (sums.s != sums.s)
-      finish_not_finite<T>(a, row, s_best);
+      finish_not_finite<T>(a, row);
     else
       finish(a, row, sums, target, s_keys, n);
     return;
@@ -386,7 +406,6 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(LogprobsArg
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_slices_kernel(LogprobsArgs a) {
   __shared__ uint64_t s_keys[kWaves * kCap];
-  __shared__ uint64_t s_best[kWaves];
   const int64_t row = blockIdx.x;
   const float target = target_of<T>(a, row);
   const int total = a.slices * a.top;
@@ -398,7 +417,7 @@ __global__ __launch_bounds__(kThreads) void join_slices_kernel(LogprobsArgs a) {
   for (int i = threadIdx.x; i < total; i += kThreads) s_keys[i] = a.ws_keys[row * total + i];
   sums = block_join(sums);  // a barrier: the keys are there
   if (sums.s != sums.s) {
-    finish_not_finite<T>(a, row, s_best);
+    finish_not_finite<T>(a, row);
     return;
   }
   // Keys of 0, the places a short slice left, are below the others, of which
