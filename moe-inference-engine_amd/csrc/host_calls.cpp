@@ -1,14 +1,17 @@
-// Host side of the short calls, compiled: paged decode of a batch and the KV
-// gather take microseconds on the device, and reading a dozen tensors'
+// Host side of the short calls, compiled: paged decode of a batch, the KV
+// gather and a serving step's operators take microseconds on the device, and reading a dozen tensors'
 // properties from Python took longer than that (5 x 1000 tokens, 8 x 96
 // float32, two launches: 17.7 -> 9.4 us a call; 1 x 2048 bfloat16 with the
 // append 18.9 -> 9.5 us; twelve layers of append and gather at 8192 tokens 188
-// -> 152 us).  Each function here takes the tensors,
+// -> 152 us; reserve of 64 rows 16.5 -> 9.4 us, rope_append of 64 tokens 15.6 ->
+// 5.1).  Each function here takes the tensors,
 // checks the form the usual calls have, allocates the results and queues the
 // launches through the library's C entry points; for any other form it returns
 // None and the caller goes through the checks written in Python, which raise
 // what is wrong.  A failed entry point's status is returned as an int.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -26,6 +29,13 @@ decltype(&mie_paged_decode_append) g_decode_append;
 decltype(&mie_paged_decode_plan) g_plan;
 decltype(&mie_paged_decode_plan_known) g_plan_known;
 decltype(&mie_kv_gather) g_gather;
+decltype(&mie_step_reserve) g_reserve;
+decltype(&mie_step_release) g_release;
+decltype(&mie_rope_append) g_rope;
+decltype(&mie_paged_extend_workspace) g_extend_workspace;
+decltype(&mie_paged_extend) g_extend;
+decltype(&mie_token_logprobs_workspace) g_logprobs_workspace;
+decltype(&mie_token_logprobs) g_logprobs;
 
 // A plain ROCm tensor: no subclass, no functorch or dispatch wrapper, storage
 // of its own device.
@@ -192,14 +202,267 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(decode, decode_append, plan, plan_known, gather): the entry points' addresses.
+// ---- a serving step's operators --------------------------------------------
+
+// A vector of n values of this type on the device (any n if negative).
+const at::Tensor* vec(PyObject* o, at::ScalarType type, c10::Device device, int64_t n) {
+  const at::Tensor* t = plain(o);
+  if (!t || t->dim() != 1 || t->scalar_type() != type || t->device() != device || !t->is_contiguous() ||
+      (n >= 0 && t->size(0) != n))
+    return nullptr;
+  return t;
+}
+
+// The launch goes to the current device, and nothing is to be recorded.
+bool usual(std::initializer_list<const at::Tensor*> tensors) {
+  const at::Tensor& t = **tensors.begin();
+  if (c10::impl::VirtualGuardImpl(t.device().type()).getDevice() != t.device()) return false;
+  if (!c10::GradMode::is_enabled()) return true;
+  for (const at::Tensor* x : tensors)
+    if (x && x->requires_grad()) return false;
+  return true;
+}
+
+bool as_double(PyObject* o, double& out) {
+  if (PyFloat_CheckExact(o)) {
+    out = PyFloat_AS_DOUBLE(o);
+    return true;
+  }
+  int64_t i;
+  if (!as_int(o, i)) return false;
+  out = static_cast<double>(i);
+  return true;
+}
+
+template <typename... T>
+PyObject* pack(T&&... tensors) {
+  PyObject* out = PyTuple_New(sizeof...(T));
+  if (!out) return nullptr;
+  Py_ssize_t i = 0;
+  (PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(std::forward<T>(tensors))), ...);
+  return out;
+}
+
+template <typename F>
+int32_t released(F launch) {
+  int32_t rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = launch();
+  Py_END_ALLOW_THREADS
+  return rc;
+}
+
+const int32_t* ints(const at::Tensor* t) { return t ? static_cast<const int32_t*>(t->data_ptr()) : nullptr; }
+int32_t* ints_out(const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+
+// Block tables [B, n]: rows of int32, not overlapping.
+const at::Tensor* table_rows(PyObject* o, c10::Device device, bool distinct) {
+  const at::Tensor* t = plain(o);
+  if (!t || t->dim() != 2 || t->scalar_type() != at::kInt || t->device() != device || t->size(0) < 1 ||
+      t->size(1) < 1 || t->stride(1) != 1 || !fits(t->size(0)) || !fits(t->size(1)) ||
+      (distinct && t->size(0) > 1 && t->stride(0) < t->size(1)))
+    return nullptr;
+  return t;
+}
+
+// reserve(free_ids, free_count, tables, context_lens, new_lens, block_size,
+//         max_tokens, stream) -> six tensors, None or a status
+PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) Py_RETURN_NONE;
+  const at::Tensor* ids = plain(a[0]);
+  int64_t block, tokens, stream;
+  if (!ids || !as_int(a[5], block) || !as_int(a[6], tokens) || !as_int(a[7], stream)) Py_RETURN_NONE;
+  const auto device = ids->device();
+  const at::Tensor* tables = table_rows(a[2], device, true);
+  if (!tables || !vec(a[0], at::kInt, device, -1)) Py_RETURN_NONE;
+  const int64_t batch = tables->size(0);
+  const at::Tensor *count = vec(a[1], at::kInt, device, 1), *lens = vec(a[3], at::kInt, device, batch),
+                   *news = vec(a[4], at::kInt, device, batch);
+  if (!count || !lens || !news || !fits(ids->size(0)) || block < 1 || !fits(block) || !fits(tokens) || !usual({ids}))
+    Py_RETURN_NONE;
+  const auto word = ids->options().requires_grad(false);
+  at::Tensor starts = at::empty({batch + 1}, word), slots = at::empty({tokens}, word.dtype(at::kLong)),
+             positions = at::empty({tokens}, word), lens_out = at::empty({batch}, word),
+             count_out = at::empty({1}, word), status = at::empty({1}, word);
+  const int32_t rc = released([&] {
+    return g_reserve(ints(ids), ids->size(0), ints(count), static_cast<int32_t*>(tables->data_ptr()),
+                     std::max(tables->stride(0), tables->size(1)), tables->size(1), ints(lens), ints(news), batch, block,
+                     tokens, ints_out(starts), static_cast<int64_t*>(slots.data_ptr()), ints_out(positions),
+                     ints_out(lens_out), ints_out(count_out), ints_out(status), reinterpret_cast<void*>(stream));
+  });
+  if (rc != MIE_OK) return PyLong_FromLong(rc);
+  return pack(starts, slots, positions, lens_out, count_out, status);
+  END_HANDLE_TH_ERRORS
+}
+
+// release(free_ids, free_count, tables, context_lens, finished, block_size,
+//         stream) -> three tensors, None or a status
+PyObject* release(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) Py_RETURN_NONE;
+  const at::Tensor* ids = plain(a[0]);
+  int64_t block, stream;
+  if (!ids || !as_int(a[5], block) || !as_int(a[6], stream)) Py_RETURN_NONE;
+  const auto device = ids->device();
+  const at::Tensor* tables = table_rows(a[2], device, true);
+  if (!tables || !vec(a[0], at::kInt, device, -1)) Py_RETURN_NONE;
+  const int64_t batch = tables->size(0);
+  const at::Tensor *count = vec(a[1], at::kInt, device, 1), *lens = vec(a[3], at::kInt, device, batch),
+                   *finished = vec(a[4], at::kBool, device, batch);
+  if (!count || !lens || !finished || !fits(ids->size(0)) || block < 1 || !fits(block) || !usual({ids})) Py_RETURN_NONE;
+  const auto word = ids->options().requires_grad(false);
+  at::Tensor lens_out = at::empty({batch}, word), count_out = at::empty({1}, word), status = at::empty({1}, word);
+  const int32_t rc = released([&] {
+    return g_release(static_cast<int32_t*>(ids->data_ptr()), ids->size(0), ints(count), ints(tables),
+                     std::max(tables->stride(0), tables->size(1)), tables->size(1), ints(lens),
+                     static_cast<const uint8_t*>(finished->data_ptr()), batch, block, ints_out(lens_out),
+                     ints_out(count_out), ints_out(status), reinterpret_cast<void*>(stream));
+  });
+  if (rc != MIE_OK) return PyLong_FromLong(rc);
+  return pack(count_out, lens_out, status);
+  END_HANDLE_TH_ERRORS
+}
+
+// rope_append(q, k, v, k_pool, v_pool, layer, slots, positions, frequencies,
+//             interleaved, factor, stream) -> q rotated, None or a status
+PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12) Py_RETURN_NONE;
+  const at::Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *kp = plain(a[3]), *vp = plain(a[4]);
+  int64_t layer, stream;
+  double factor;
+  if (!q || !k || !v || !kp || !vp || !as_int(a[5], layer) || !PyBool_Check(a[9]) || !as_double(a[10], factor) ||
+      !as_int(a[11], stream))
+    Py_RETURN_NONE;
+  const int code = dtype_code(kp->scalar_type());
+  const auto device = kp->device();
+  if (code < 0 || q->dim() != 3 || k->dim() != 3 || kp->dim() != 5 || vp->sizes() != kp->sizes() ||
+      !kp->is_contiguous() || !vp->is_contiguous() || vp->device() != device || vp->scalar_type() != kp->scalar_type())
+    Py_RETURN_NONE;
+  const auto ps = kp->sizes();
+  const int64_t tokens = q->size(0), heads = q->size(1), blocks = ps[1], kv_heads = ps[2], block = ps[3], dim = ps[4];
+  for (const at::Tensor* t : {q, k, v})
+    if (t->scalar_type() != kp->scalar_type() || t->device() != device) Py_RETURN_NONE;
+  if (q->size(2) != dim || q->stride(2) != 1 || k->size(0) != tokens || k->size(1) != kv_heads || k->size(2) != dim ||
+      k->stride(2) != 1 || v->sizes() != k->sizes() || v->strides() != k->strides() || layer < 0 || layer >= ps[0] ||
+      !fits(tokens) || !fits(heads) || !fits(blocks) || !fits(block) || !fits(dim))
+    Py_RETURN_NONE;
+  const at::Tensor *slots = vec(a[6], at::kLong, device, tokens), *positions = vec(a[7], at::kInt, device, tokens),
+                   *freq = vec(a[8], at::kDouble, device, -1);
+  if (!slots || !positions || !freq || freq->size(0) > dim || !usual({q, k, v, freq})) Py_RETURN_NONE;
+  at::Tensor out = at::empty({tokens, heads, dim}, q->options().requires_grad(false));
+  const int64_t tile = block * dim, offset = layer * blocks * kv_heads * tile * kp->element_size();
+  const int32_t rc = released([&] {
+    return g_rope(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), v->data_ptr(), k->stride(0), k->stride(1),
+                  static_cast<char*>(kp->data_ptr()) + offset, static_cast<char*>(vp->data_ptr()) + offset,
+                  kv_heads * tile, tile, blocks, static_cast<const int64_t*>(slots->data_ptr()), ints(positions),
+                  static_cast<const double*>(freq->data_ptr()), 2 * freq->size(0), a[9] == Py_True,
+                  static_cast<float>(factor), tokens, heads, kv_heads, dim, block, out.data_ptr(), heads * dim, dim,
+                  code, reinterpret_cast<void*>(stream));
+  });
+  if (rc != MIE_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// extend(q, k_pool, v_pool, layer, tables, starts, context_lens, max_new,
+//        max_len, scale, softcap, slopes, window, prefix_lens, stream) -> out,
+// None or a status.  scale a float or None; slopes, prefix_lens may be None.
+PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 15) Py_RETURN_NONE;
+  const at::Tensor *q = plain(a[0]), *kp = plain(a[1]), *vp = plain(a[2]);
+  int64_t layer, max_new, max_len, window, stream;
+  double scale = 0, softcap;
+  if (!q || !kp || !vp || !as_int(a[3], layer) || !as_int(a[7], max_new) || !as_int(a[8], max_len) ||
+      (a[9] != Py_None && !as_double(a[9], scale)) || !as_double(a[10], softcap) || !as_int(a[12], window) ||
+      !as_int(a[14], stream))
+    Py_RETURN_NONE;
+  const int code = dtype_code(q->scalar_type());
+  const auto device = q->device();
+  if (code < 0 || q->dim() != 3 || kp->dim() != 5 || vp->sizes() != kp->sizes() || !kp->is_contiguous() ||
+      !vp->is_contiguous() || kp->device() != device || vp->device() != device ||
+      kp->scalar_type() != q->scalar_type() || vp->scalar_type() != q->scalar_type())
+    Py_RETURN_NONE;
+  const auto ps = kp->sizes();
+  const int64_t tokens = q->size(0), heads = q->size(1), blocks = ps[1], kv_heads = ps[2], block = ps[3], dim = ps[4];
+  const int64_t align = 16 / q->element_size();
+  const at::Tensor* tables = table_rows(a[4], device, false);
+  if (!tables || tokens < 1 || q->size(2) != dim || q->stride(2) != 1 || q->stride(0) % align ||
+      q->stride(1) % align || reinterpret_cast<uintptr_t>(q->data_ptr()) % 16 || layer < 0 || layer >= ps[0] ||
+      kv_heads < 1 || heads < 1 || heads % kv_heads || !fits(tokens) || !fits(heads) || !fits(blocks) || !fits(block) ||
+      !fits(dim) || !fits(max_new) || !fits(max_len) || !fits(window) || !(softcap >= 0 && std::isfinite(softcap)))
+    Py_RETURN_NONE;
+  const int64_t batch = tables->size(0);
+  const at::Tensor *starts = vec(a[5], at::kInt, device, batch + 1), *lens = vec(a[6], at::kInt, device, batch),
+                   *slopes = nullptr, *prefix = nullptr;
+  if (!starts || !lens || (a[11] != Py_None && !(slopes = vec(a[11], at::kFloat, device, heads))) ||
+      (a[13] != Py_None && !(prefix = vec(a[13], at::kInt, device, batch))) || !usual({q, kp, vp, slopes}))
+    Py_RETURN_NONE;
+  if (a[9] == Py_None) scale = 1.0 / std::sqrt(static_cast<double>(dim));
+  const int64_t bytes = g_extend_workspace(tokens, batch, max_new, max_len, window, heads, kv_heads, dim, code);
+  if (bytes < 0) Py_RETURN_NONE;  // refused: the other path says why
+  at::Tensor out = at::empty({tokens, heads, dim}, q->options().requires_grad(false)), ws;
+  if (bytes > 0) ws = at::empty({bytes}, q->options().dtype(at::kByte).requires_grad(false));
+  const int64_t tile = block * dim, offset = layer * blocks * kv_heads * tile * kp->element_size();
+  const int32_t rc = released([&] {
+    return g_extend(q->data_ptr(), q->stride(0), q->stride(1), static_cast<const char*>(kp->data_ptr()) + offset,
+                    static_cast<const char*>(vp->data_ptr()) + offset, kv_heads * tile, tile, blocks, ints(tables),
+                    std::max(tables->stride(0), tables->size(1)), tables->size(1), ints(starts), ints(lens), tokens,
+                    batch, max_new, max_len, heads, kv_heads, dim, block, static_cast<float>(scale),
+                    static_cast<float>(softcap), slopes ? static_cast<const float*>(slopes->data_ptr()) : nullptr,
+                    window, ints(prefix), out.data_ptr(), heads * dim, dim, bytes > 0 ? ws.data_ptr() : nullptr, bytes,
+                    code, reinterpret_cast<void*>(stream));
+  });
+  if (rc != MIE_OK) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// logprobs(logits, tokens, top, stream) -> (logprobs, entropy, top_logprobs,
+// top_tokens), None or a status
+PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) Py_RETURN_NONE;
+  const at::Tensor* x = plain(a[0]);
+  int64_t top, stream;
+  if (!x || !as_int(a[2], top) || !as_int(a[3], stream)) Py_RETURN_NONE;
+  const int code = dtype_code(x->scalar_type());
+  if (code < 0 || x->dim() != 2) Py_RETURN_NONE;
+  const int64_t rows = x->size(0), vocab = x->size(1);
+  const at::Tensor* tokens = vec(a[1], at::kLong, x->device(), rows);
+  if (!tokens || vocab < 1 || x->stride(1) != 1 || (rows > 1 && x->stride(0) < vocab) || !fits(rows) || !fits(vocab) ||
+      top < 0 || top > vocab || !fits(top) || !usual({x}))
+    Py_RETURN_NONE;
+  const int64_t bytes = g_logprobs_workspace(rows, vocab, top);
+  const auto real = x->options().dtype(at::kFloat).requires_grad(false);
+  at::Tensor given = at::empty({rows}, real), entropy = at::empty({rows}, real), best = at::empty({rows, top}, real),
+             ids = at::empty({rows, top}, real.dtype(at::kLong)), ws;
+  if (bytes > 0) ws = at::empty({bytes}, real.dtype(at::kByte));
+  const int32_t rc = released([&] {
+    return g_logprobs(x->data_ptr(), std::max(x->stride(0), vocab), rows, vocab,
+                      static_cast<const int64_t*>(tokens->data_ptr()), top, static_cast<float*>(given.data_ptr()),
+                      static_cast<float*>(entropy.data_ptr()), static_cast<float*>(best.data_ptr()),
+                      static_cast<int64_t*>(ids.data_ptr()), bytes > 0 ? ws.data_ptr() : nullptr, bytes, code,
+                      reinterpret_cast<void*>(stream));
+  });
+  if (rc != MIE_OK) return PyLong_FromLong(rc);
+  return pack(given, entropy, best, ids);
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(decode, decode_append, plan, plan_known, gather, reserve, release,
+// rope_append, extend_workspace, extend, logprobs_workspace, logprobs): the
+// entry points' addresses.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* p[5];
-  if (n != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind takes five addresses");
+  constexpr int kEntries = 12;
+  void* p[kEntries];
+  if (n != kEntries) {
+    PyErr_SetString(PyExc_TypeError, "bind takes twelve addresses");
     return nullptr;
   }
-  for (int i = 0; i < 5; ++i) {
+  for (int i = 0; i < kEntries; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (!p[i]) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
@@ -211,12 +474,24 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g_plan = reinterpret_cast<decltype(g_plan)>(p[2]);
   g_plan_known = reinterpret_cast<decltype(g_plan_known)>(p[3]);
   g_gather = reinterpret_cast<decltype(g_gather)>(p[4]);
+  g_reserve = reinterpret_cast<decltype(g_reserve)>(p[5]);
+  g_release = reinterpret_cast<decltype(g_release)>(p[6]);
+  g_rope = reinterpret_cast<decltype(g_rope)>(p[7]);
+  g_extend_workspace = reinterpret_cast<decltype(g_extend_workspace)>(p[8]);
+  g_extend = reinterpret_cast<decltype(g_extend)>(p[9]);
+  g_logprobs_workspace = reinterpret_cast<decltype(g_logprobs_workspace)>(p[10]);
+  g_logprobs = reinterpret_cast<decltype(g_logprobs)>(p[11]);
   Py_RETURN_NONE;
 }
 
 PyMethodDef g_methods[] = {
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(decode)), METH_FASTCALL, nullptr},
     {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gather)), METH_FASTCALL, nullptr},
+    {"reserve", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(reserve)), METH_FASTCALL, nullptr},
+    {"release", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(release)), METH_FASTCALL, nullptr},
+    {"rope_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(rope_append)), METH_FASTCALL, nullptr},
+    {"extend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(extend)), METH_FASTCALL, nullptr},
+    {"logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(logprobs)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

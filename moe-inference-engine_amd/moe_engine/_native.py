@@ -298,12 +298,22 @@ def _open_host():
                       RuntimeWarning, stacklevel=2)
         return None
     entry_points = (_LIB.mie_paged_decode, _LIB.mie_paged_decode_append, _LIB.mie_paged_decode_plan,
-                    _LIB.mie_paged_decode_plan_known, _LIB.mie_kv_gather)
+                    _LIB.mie_paged_decode_plan_known, _LIB.mie_kv_gather, _LIB.mie_step_reserve,
+                    _LIB.mie_step_release, _LIB.mie_rope_append, _LIB.mie_paged_extend_workspace,
+                    _LIB.mie_paged_extend, _LIB.mie_token_logprobs_workspace, _LIB.mie_token_logprobs)
     _host_calls.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in entry_points))
     return _host_calls
 
 
 HOST = _open_host()
+
+
+def host_result(got, what: str):
+    """A compiled call's answer: its result, None where it left the call to
+    the Python path, or the error a failed entry point's status stands for."""
+    if type(got) is int:
+        check(got, what)
+    return got
 
 
 def lib():

@@ -322,6 +322,14 @@ def reserve(
     the lengths and the free count come back unchanged.  The inputs are not
     advanced: carry context_lens and free_count to the next call.
     """
+    host = _native.HOST
+    if host is not None and free_ids.is_cuda:
+        # The usual form in one compiled call; None for any other, which the
+        # checks below take (or refuse).
+        got = _native.host_result(host.reserve(free_ids, free_count, block_tables, context_lens, new_lens, block_size,
+                                               max_tokens, _native.stream_of(free_ids)), "mie_step_reserve")
+        if got is not None:
+            return StepSlots(*got)
     batch, device = _check_step(free_ids, free_count, block_tables, context_lens, block_size)
     if new_lens.dtype != torch.int32 or new_lens.shape != (batch,) or new_lens.device != device \
             or not new_lens.is_contiguous():
@@ -360,6 +368,12 @@ def release(
     launch: free_ids is written from free_count[0] on, finished sequences'
     lengths become 0.  All or nothing, like reserve.  Each sequence's blocks
     must be its own."""
+    host = _native.HOST
+    if host is not None and free_ids.is_cuda:
+        got = _native.host_result(host.release(free_ids, free_count, block_tables, context_lens, finished, block_size,
+                                               _native.stream_of(free_ids)), "mie_step_release")
+        if got is not None:
+            return StepRelease(*got)
     batch, device = _check_step(free_ids, free_count, block_tables, context_lens, block_size)
     if finished.dtype != torch.bool or finished.shape != (batch,) or finished.device != device \
             or not finished.is_contiguous():
@@ -454,6 +468,12 @@ def rope_append(
     multiplied by `factor`.  H_kv and D are the pool's; D and R are even.
     Two tokens must not share a slot.
     """
+    host = _native.HOST
+    if host is not None and out is None and q.is_cuda:
+        got = _native.host_result(host.rope_append(q, k, v, k_pool, v_pool, layer_idx, slots, positions, frequencies,
+                                                   interleaved, factor, _native.stream_of(q)), "mie_rope_append")
+        if got is not None:
+            return got
     _check_pools(k_pool, v_pool)
     kl, vl = _layer(k_pool, layer_idx), _layer(v_pool, layer_idx)
     nb, kv_heads, block_size, head_dim = kl.shape

@@ -382,6 +382,13 @@ def extend_batched(
 
     float32 or bfloat16, D one of EXTEND_HEAD_DIMS; float32 sums and softmax.
     """
+    host = _native.HOST
+    if host is not None and out is None and q.is_cuda:
+        got = _native.host_result(host.extend(q, k_pool, v_pool, layer_idx, block_tables, starts, context_lens,
+                                              max_new_tokens, max_context_len, scale, softcap, slopes, window,
+                                              prefix_lens, _native.stream_of(q)), "mie_paged_extend")
+        if got is not None:
+            return got
     if q.dim() != 3 or k_pool.dim() != 5 or k_pool.shape != v_pool.shape:
         raise ValueError("q must be [tokens, heads, head_dim], the pools [layers, blocks, heads, block_size, head_dim]")
     if not 0 <= layer_idx < k_pool.shape[0]:

@@ -241,6 +241,11 @@ def token_logprobs(logits, tokens=None, top: int = 0) -> TokenLogprobs:
     values with their tokens, the lower token first among equals, NaN the
     largest.  float32 results.  -inf marks a token that cannot be; a row of
     nothing else, or with a NaN or +inf, has NaN log probabilities and entropy."""
+    host = _native.HOST
+    if host is not None and tokens is not None and logits.is_cuda:
+        got = _native.host_result(host.logprobs(logits, tokens, top, _native.stream_of(logits)), "mie_token_logprobs")
+        if got is not None:
+            return TokenLogprobs(*got)
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[1] < 1:
         raise ValueError("logits must be [rows, vocab] in float32 or bfloat16")
     if not _native.is_rocm_device(logits):
