@@ -40,13 +40,24 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kRows = mie::extend::kFewRows;
 
+// A load of data that is read once, in whole cache lines per instruction, goes
+// around the caches: V's (K's operands are half lines).
+template <bool ONCE, typename V>
+__device__ __forceinline__ V fetch(const V* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(p);
+  return *p;
+}
+
 // V's operands of one 64- or 32-dim group for 32 keys, and their products.
 // Lane (i, g): keys 16 t + 4 g + r (t < 2, r < 4), dims VEC i .. VEC i + VEC - 1.
 template <typename T, int VEC> struct Values;
 template <int VEC> struct Values<float, VEC> {
   typedef float vec __attribute__((ext_vector_type(VEC)));
   vec v[2][4];
-  __device__ __forceinline__ void load(int t, int r, const char* p) { v[t][r] = *reinterpret_cast<const vec*>(p); }
+  template <bool ONCE>
+  __device__ __forceinline__ void load(int t, int r, const char* p) {
+    v[t][r] = fetch<ONCE>(reinterpret_cast<const vec*>(p));
+  }
   __device__ __forceinline__ bool not_finite() const {
     bool any = false;
 #pragma unroll
@@ -69,13 +80,14 @@ template <int VEC> struct Values<float, VEC> {
 };
 template <int VEC> struct Values<uint16_t, VEC> {
   uint32_t v[2][4][VEC / 2];
+  template <bool ONCE>
   __device__ __forceinline__ void load(int t, int r, const char* p) {
     if constexpr (VEC == 4) {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      const u32x2 x = fetch<ONCE>(reinterpret_cast<const u32x2*>(p));
       v[t][r][0] = x.x;
       v[t][r][1] = x.y;
     } else {
-      v[t][r][0] = *reinterpret_cast<const uint32_t*>(p);
+      v[t][r][0] = fetch<ONCE>(reinterpret_cast<const uint32_t*>(p));
     }
   }
   __device__ __forceinline__ bool not_finite() const {
@@ -118,8 +130,9 @@ __device__ __forceinline__ int dim_of(int n, int r, int g) {
   return n < G4 * 4 ? n / 4 * 64 + g * 16 + r * 4 + n % 4 : G4 * 64 + (n - G4 * 4) / 2 * 32 + g * 8 + r * 2 + n % 2;
 }
 
-// grid = tiles x parts x kv_heads, the K/V head fastest.
-template <typename T, int D>
+// grid = tiles x parts x kv_heads, the K/V head fastest.  ONCE: a sequence has
+// one tile, so nobody else reads its keys.
+template <typename T, int D, bool ONCE>
 __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_rows_kernel(Args a) {
   constexpr int NCH = D * static_cast<int>(sizeof(T)) / 64;  // 64-byte pieces of a row
   constexpr int G4 = D / 64, G2 = D % 64 / 32;               // 64- and 32-dim groups
@@ -195,9 +208,9 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_rows
       for (int r = 0; r < 4; ++r) {
         const char* v = v_head + s_off[wave][buffer][t * 16 + g * 4 + r];
 #pragma unroll
-        for (int n = 0; n < G4; ++n) v4[n].load(t, r, v + (n * 64 + i * 4) * sizeof(T));
+        for (int n = 0; n < G4; ++n) v4[n].template load<ONCE>(t, r, v + (n * 64 + i * 4) * sizeof(T));
 #pragma unroll
-        for (int n = 0; n < G2; ++n) v2[n].load(t, r, v + (G4 * 64 + n * 32 + i * 2) * sizeof(T));
+        for (int n = 0; n < G2; ++n) v2[n].template load<ONCE>(t, r, v + (G4 * 64 + n * 32 + i * 2) * sizeof(T));
       }
     f32x4 s[2];
 #pragma unroll
@@ -334,42 +347,67 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_rows
   }
 }
 
-// Joins the partitions of 16 of a tile's ROWS rows.  grid = (tiles x kv_heads, ROWS / 16).
+// Joins the partitions of a row.  grid = (tiles x kv_heads, ROWS).  The
+// workgroup's threads are D / 4 columns of four dims by 1024 / D partitions at
+// a time; every wave sees all maxima, so no exchange comes before the sums.
 template <typename T, int D, int ROWS>
 __global__ __launch_bounds__(256) void extend_join_kernel(Args a) {
-  const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
+  constexpr int kCols = D / 4, kAtOnce = 256 / kCols;
+  __shared__ __align__(16) f32x4 s_v[kAtOnce][kCols];
+  __shared__ float s_sum[kAtOnce];
+  const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, in_tile = blockIdx.y;
   const Place p = mie::extend::find_place<ROWS>(a, tile);
-  if (p.b < 0) return;
+  const int r = p.row0 + in_tile;
+  if (p.b < 0 || r >= p.rows) return;
   const int parts = mie::extend::parts_of(a, p);
   if (parts == 1) return;
+  const int col = threadIdx.x % kCols, at = threadIdx.x / kCols;
   const int64_t piece = (static_cast<int64_t>(tile) * a.kv_heads + kvh) * a.parts;
-  for (int e = threadIdx.x; e < 16 * (D / 4); e += 256) {
-    const int in_tile = blockIdx.y * 16 + e / (D / 4), c = e % (D / 4) * 4;
-    const int r = p.row0 + in_tile;
-    if (r >= p.rows) break;
-    const float* ml = a.ws_ml + (piece * ROWS + in_tile) * 2;
-    const float* acc = a.ws_acc + (piece * ROWS + in_tile) * D + c;
-    float top = -INFINITY;
-    for (int j = 0; j < parts; ++j) top = fmaxf(top, ml[j * ROWS * 2]);
-    float sum = 0.f;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < parts; ++j) {
-      const float mj = ml[j * ROWS * 2];
+  const float* ml = a.ws_ml + (piece * ROWS + in_tile) * 2;
+  const float* acc = a.ws_acc + (piece * ROWS + in_tile) * D + col * 4;
+  float top = -INFINITY;
+  for (int j = threadIdx.x & 63; j < parts; j += 64) top = fmaxf(top, ml[static_cast<int64_t>(j) * ROWS * 2]);
+  top = mie::wave_max(top);
+  float sum = 0.f;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (at < kAtOnce) {  // 24 columns leave 16 threads over
+#pragma unroll 4
+    for (int j = at; j < parts; j += kAtOnce) {
+      const float mj = ml[static_cast<int64_t>(j) * ROWS * 2];
       const float f = mj == -INFINITY ? 1.f : mie::fast_exp2(mj - top);
-      sum += f * ml[j * ROWS * 2 + 1];
+      sum += f * ml[static_cast<int64_t>(j) * ROWS * 2 + 1];
       v += f * *reinterpret_cast<const f32x4*>(acc + static_cast<int64_t>(j) * ROWS * D);
     }
-    v = sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v / sum;
-    const int t = a.group.div(r);
-    Mem<T>::put4(reinterpret_cast<T*>(a.out + (p.start + t) * a.out_st +
-                                      (kvh * a.group.d + r - t * a.group.d) * a.out_sh) + c, v);
+    s_v[at][col] = v;
+    if (col == 0) s_sum[at] = sum;
   }
+  __syncthreads();
+  if (at != 0) return;
+  v = s_v[0][col];
+  sum = s_sum[0];
+#pragma unroll
+  for (int j = 1; j < kAtOnce; ++j) {
+    v += s_v[j][col];
+    sum += s_sum[j];
+  }
+  v = sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v / sum;
+  const int t = a.group.div(r);
+  Mem<T>::put4(reinterpret_cast<T*>(a.out + (p.start + t) * a.out_st +
+                                    (kvh * a.group.d + r - t * a.group.d) * a.out_sh) + col * 4, v);
 }
 
 // ---- host ------------------------------------------------------------------
 
-constexpr int kMinPart = 256;       // keys of the smallest partition
-constexpr int kGroupsWanted = 1024;  // workgroups that fill the 256 CUs
+// Workgroups that the keys are split for, and the keys of the smallest
+// partition: in general, and where a sequence has one tile, so that its keys
+// are read once and reading them is the work (its partitions also even out
+// ragged lengths).  Measured on MI355X, us: 64 sequences of 512 to 8192 tokens
+// (32 heads over 8 x 128, bfloat16) 240 with 2048 workgroups, 216 with 4096,
+// 216 with 8192, (12 x 64) 187, 155, 153; 1 x 2048 (12 x 64) 10.2 with
+// partitions of 256, 8.8 with 128, 13.5 with 512; 1 x 100000 76 with 256 and
+// 87 with 128 (many more to join).
+constexpr int kGroups = 1024, kMinPart = 256;
+constexpr int kGroupsOnce = 4096, kMinPartOnce = 128;
 
 struct Plan {
   int rows;  // of a tile
@@ -400,7 +438,7 @@ bool many_rows(int64_t tokens, int max_new, int64_t keys, int group, int kv_head
 }
 
 // Row tiles: as many as the batch can have (the lengths are on the device).
-// The keys are split until the tiles make kGroupsWanted workgroups.
+// The keys are split until the tiles make the workgroups wanted.
 Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int group, int kv_heads, int head_dim,
                int dtype) {
   Plan p;
@@ -414,8 +452,10 @@ Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int 
   // Keys a tile can see: all, or a window back from each of its tokens.
   const int64_t span = (rows + group - 1) / group + 1;
   const int64_t range = window > 0 ? std::min<int64_t>(max_len, static_cast<int64_t>(window) + span + 32) : max_len;
-  const int64_t want = std::max<int64_t>(1, kGroupsWanted / (p.tiles * kv_heads));
-  const int64_t parts = std::min<int64_t>(want, (range + kMinPart - 1) / kMinPart);
+  const bool once = static_cast<int64_t>(max_new) * group <= kFewRows;
+  const int min_part = once ? kMinPartOnce : kMinPart;
+  const int64_t want = std::max<int64_t>(1, (once ? kGroupsOnce : kGroups) / (p.tiles * kv_heads));
+  const int64_t parts = std::min<int64_t>(want, (range + min_part - 1) / min_part);
   if (parts <= 1) {
     p.parts = 1;
     p.part_keys = INT_MAX;
@@ -449,15 +489,17 @@ int32_t check_shape(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_
 template <typename T, int D>
 void launch(const Args& a, const Plan& plan, hipStream_t st) {
   const uint32_t rows = static_cast<uint32_t>(plan.tiles * a.kv_heads);
-  if (plan.rows == kFewRows)
-    extend_rows_kernel<T, D><<<rows * plan.parts, 256, 0, st>>>(a);
-  else
+  if (plan.rows == kTileRows)
     mie::extend::launch_tiles(a, sizeof(T) == 4 ? MIE_DTYPE_F32 : MIE_DTYPE_BF16, D, st);
+  else if (static_cast<int64_t>(a.max_new) * a.group.d <= kFewRows)
+    extend_rows_kernel<T, D, true><<<rows * plan.parts, 256, 0, st>>>(a);
+  else
+    extend_rows_kernel<T, D, false><<<rows * plan.parts, 256, 0, st>>>(a);
   if (plan.parts == 1) return;
   if (plan.rows == kFewRows)
-    extend_join_kernel<T, D, kFewRows><<<dim3(rows), 256, 0, st>>>(a);
+    extend_join_kernel<T, D, kFewRows><<<dim3(rows, kFewRows), 256, 0, st>>>(a);
   else
-    extend_join_kernel<T, D, kTileRows><<<dim3(rows, kTileRows / 16), 256, 0, st>>>(a);
+    extend_join_kernel<T, D, kTileRows><<<dim3(rows, kTileRows), 256, 0, st>>>(a);
 }
 
 template <typename T>
