@@ -347,7 +347,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_rows
   }
 }
 
-// Joins the partitions of a row.  grid = (tiles x kv_heads, ROWS).  The
+// Joins the partitions of a row.  grid = (tiles x kv_heads, rows of a tile).  The
 // workgroup's threads are D / 4 columns of four dims by 1024 / D partitions at
 // a time; every wave sees all maxima, so no exchange comes before the sums.
 template <typename T, int D, int ROWS>
@@ -496,10 +496,11 @@ void launch(const Args& a, const Plan& plan, hipStream_t st) {
   else
     extend_rows_kernel<T, D, false><<<rows * plan.parts, 256, 0, st>>>(a);
   if (plan.parts == 1) return;
+  const dim3 grid(rows, static_cast<uint32_t>(std::min<int64_t>(plan.rows, static_cast<int64_t>(a.max_new) * a.group.d)));
   if (plan.rows == kFewRows)
-    extend_join_kernel<T, D, kFewRows><<<dim3(rows, kFewRows), 256, 0, st>>>(a);
+    extend_join_kernel<T, D, kFewRows><<<grid, 256, 0, st>>>(a);
   else
-    extend_join_kernel<T, D, kTileRows><<<dim3(rows, kTileRows), 256, 0, st>>>(a);
+    extend_join_kernel<T, D, kTileRows><<<grid, 256, 0, st>>>(a);
 }
 
 template <typename T>

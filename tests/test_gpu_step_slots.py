@@ -54,9 +54,10 @@ def check_reserve(c):
     (1, 0, 0, 1, 1, 16), (1, 0, 0, 0, 0, 16), (1, 15, 15, 1, 1, 16), (1, 16, 16, 1, 1, 16), (3, 0, 40, 0, 5, 16),
     (64, 0, 600, 1, 1, 16), (64, 0, 600, 0, 1, 1), (65, 0, 90, 0, 70, 7), (255, 0, 50, 0, 3, 8),
     (256, 0, 50, 0, 3, 32), (257, 0, 50, 0, 3, 16), (1000, 0, 100, 0, 40, 16), (5, 0, 9000, 0, 9000, 16),
-    (2, 0, 0, 3000, 5000, 1), (8192, 0, 3, 0, 2, 2),
+    (2, 0, 0, 2500, 5000, 1), (8192, 0, 3, 0, 2, 2),
+    (500, 0, 100, 0, 600, 16), (3, 0, 7, 20000, 30000, 16), (8192, 0, 40, 0, 30, 16), (90, 0, 0, 0, 5000, 7),
 ], ids=str)
-@pytest.mark.parametrize("pad", [0, 300])
+@pytest.mark.parametrize("pad", [0, 300, 301])
 def test_reserve_is_the_host_allocators(args, pad):
     print_case("reserve", args, pad)
     step = check_reserve(case(*args, seed=sum(args), pad=pad))
