@@ -252,6 +252,15 @@ int32_t released(F launch) {
   return rc;
 }
 
+// n values of one allocation from the at-th on, as a tensor of their own: an
+// at::empty costs 0.7 us, this 0.1.
+at::Tensor piece(const at::Tensor& whole, int64_t at, int64_t n) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+  impl->set_storage_offset(at);
+  impl->set_sizes_contiguous({n});
+  return at::Tensor(std::move(impl));
+}
+
 const int32_t* ints(const at::Tensor* t) { return t ? static_cast<const int32_t*>(t->data_ptr()) : nullptr; }
 int32_t* ints_out(const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
 
@@ -282,9 +291,11 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!count || !lens || !news || !fits(ids->size(0)) || block < 1 || !fits(block) || !fits(tokens) || !usual({ids}))
     Py_RETURN_NONE;
   const auto word = ids->options().requires_grad(false);
-  at::Tensor starts = at::empty({batch + 1}, word), slots = at::empty({tokens}, word.dtype(at::kLong)),
-             positions = at::empty({tokens}, word), lens_out = at::empty({batch}, word),
-             count_out = at::empty({1}, word), status = at::empty({1}, word);
+  // One allocation of words, the positions first (16-byte aligned).
+  at::Tensor slots = at::empty({tokens}, word.dtype(at::kLong)), words = at::empty({tokens + 2 * batch + 3}, word);
+  at::Tensor positions = piece(words, 0, tokens), starts = piece(words, tokens, batch + 1),
+             lens_out = piece(words, tokens + batch + 1, batch), count_out = piece(words, tokens + 2 * batch + 1, 1),
+             status = piece(words, tokens + 2 * batch + 2, 1);
   const int32_t rc = released([&] {
     return g_reserve(ints(ids), ids->size(0), ints(count), static_cast<int32_t*>(tables->data_ptr()),
                      std::max(tables->stride(0), tables->size(1)), tables->size(1), ints(lens), ints(news), batch, block,
@@ -312,7 +323,8 @@ PyObject* release(PyObject*, PyObject* const* a, Py_ssize_t n) {
                    *finished = vec(a[4], at::kBool, device, batch);
   if (!count || !lens || !finished || !fits(ids->size(0)) || block < 1 || !fits(block) || !usual({ids})) Py_RETURN_NONE;
   const auto word = ids->options().requires_grad(false);
-  at::Tensor lens_out = at::empty({batch}, word), count_out = at::empty({1}, word), status = at::empty({1}, word);
+  at::Tensor words = at::empty({batch + 2}, word);
+  at::Tensor lens_out = piece(words, 0, batch), count_out = piece(words, batch, 1), status = piece(words, batch + 1, 1);
   const int32_t rc = released([&] {
     return g_release(static_cast<int32_t*>(ids->data_ptr()), ids->size(0), ints(count), ints(tables),
                      std::max(tables->stride(0), tables->size(1)), tables->size(1), ints(lens),
