@@ -347,49 +347,62 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_rows
   }
 }
 
-// Joins the partitions of a row.  grid = (tiles x kv_heads, rows of a tile).  The
-// workgroup's threads are D / 4 columns of four dims by 1024 / D partitions at
-// a time; every wave sees all maxima, so no exchange comes before the sums.
+// Partitions that are summed side by side, a power of two: many where there
+// are many partitions (then few rows), so that a column's chain is short.
+template <int D>
+constexpr int join_lanes(int parts) {
+  int lanes = 1;
+  while (lanes * 2 <= parts && lanes * 2 <= 1024 / D) lanes *= 2;
+  return lanes;
+}
+
+// Joins the partitions of a tile's rows in one pass over them, with a running
+// maximum like the kernels'.  A row takes D / 4 columns of four dims by `lanes`
+// partitions at a time, a workgroup as many rows as that leaves.
+// grid = (tiles x kv_heads, ceil(rows of a tile / per group)).
 template <typename T, int D, int ROWS>
-__global__ __launch_bounds__(256) void extend_join_kernel(Args a) {
-  constexpr int kCols = D / 4, kAtOnce = 256 / kCols;
+__global__ __launch_bounds__(256) void extend_join_kernel(Args a, int lanes) {
+  constexpr int kCols = D / 4, kAtOnce = 256 / kCols;  // 24 columns leave 16 threads over
   __shared__ __align__(16) f32x4 s_v[kAtOnce][kCols];
-  __shared__ float s_sum[kAtOnce];
-  const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, in_tile = blockIdx.y;
+  __shared__ float s_top[kAtOnce], s_sum[kAtOnce];
+  const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
   const Place p = mie::extend::find_place<ROWS>(a, tile);
-  const int r = p.row0 + in_tile;
-  if (p.b < 0 || r >= p.rows) return;
+  if (p.b < 0) return;
   const int parts = mie::extend::parts_of(a, p);
   if (parts == 1) return;
   const int col = threadIdx.x % kCols, at = threadIdx.x / kCols;
+  const int lane = at & (lanes - 1), in_tile = blockIdx.y * (kAtOnce / lanes) + at / lanes;
+  const int r = p.row0 + in_tile;
+  const bool have = at / lanes < kAtOnce / lanes && in_tile < ROWS && r < p.rows;
   const int64_t piece = (static_cast<int64_t>(tile) * a.kv_heads + kvh) * a.parts;
-  const float* ml = a.ws_ml + (piece * ROWS + in_tile) * 2;
-  const float* acc = a.ws_acc + (piece * ROWS + in_tile) * D + col * 4;
-  float top = -INFINITY;
-  for (int j = threadIdx.x & 63; j < parts; j += 64) top = fmaxf(top, ml[static_cast<int64_t>(j) * ROWS * 2]);
-  top = mie::wave_max(top);
-  float sum = 0.f;
+  float top = -INFINITY, sum = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (at < kAtOnce) {  // 24 columns leave 16 threads over
+  // A part without seen keys has no weight: sum and values 0 (or NaN, kept).
+  auto take = [&](float m, float s, f32x4 x) {
+    const float to = fmaxf(top, m);
+    const float f = m == -INFINITY ? 1.f : mie::fast_exp2(m - to);
+    const float g = top == -INFINITY ? 1.f : mie::fast_exp2(top - to);
+    sum = sum * g + s * f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = v[e] * g + x[e] * f;
+    top = to;
+  };
+  if (have) {
+    const float* ml = a.ws_ml + (piece * ROWS + in_tile) * 2;
+    const float* acc = a.ws_acc + (piece * ROWS + in_tile) * D + col * 4;
 #pragma unroll 4
-    for (int j = at; j < parts; j += kAtOnce) {
-      const float mj = ml[static_cast<int64_t>(j) * ROWS * 2];
-      const float f = mj == -INFINITY ? 1.f : mie::fast_exp2(mj - top);
-      sum += f * ml[static_cast<int64_t>(j) * ROWS * 2 + 1];
-      v += f * *reinterpret_cast<const f32x4*>(acc + static_cast<int64_t>(j) * ROWS * D);
-    }
+    for (int j = lane; j < parts; j += lanes)
+      take(ml[static_cast<int64_t>(j) * ROWS * 2], ml[static_cast<int64_t>(j) * ROWS * 2 + 1],
+           *reinterpret_cast<const f32x4*>(acc + static_cast<int64_t>(j) * ROWS * D));
     s_v[at][col] = v;
-    if (col == 0) s_sum[at] = sum;
+    if (col == 0) {
+      s_top[at] = top;
+      s_sum[at] = sum;
+    }
   }
   __syncthreads();
-  if (at != 0) return;
-  v = s_v[0][col];
-  sum = s_sum[0];
-#pragma unroll
-  for (int j = 1; j < kAtOnce; ++j) {
-    v += s_v[j][col];
-    sum += s_sum[j];
-  }
+  if (!have || lane != 0) return;
+  for (int j = 1; j < lanes; ++j) take(s_top[at + j], s_sum[at + j], s_v[at + j][col]);
   v = sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v / sum;
   const int t = a.group.div(r);
   Mem<T>::put4(reinterpret_cast<T*>(a.out + (p.start + t) * a.out_st +
@@ -496,11 +509,13 @@ void launch(const Args& a, const Plan& plan, hipStream_t st) {
   else
     extend_rows_kernel<T, D, false><<<rows * plan.parts, 256, 0, st>>>(a);
   if (plan.parts == 1) return;
-  const dim3 grid(rows, static_cast<uint32_t>(std::min<int64_t>(plan.rows, static_cast<int64_t>(a.max_new) * a.group.d)));
+  const int lanes = join_lanes<D>(plan.parts), per_group = 256 / (D / 4) / lanes;
+  const int64_t most = std::min<int64_t>(plan.rows, static_cast<int64_t>(a.max_new) * a.group.d);
+  const dim3 grid(rows, static_cast<uint32_t>((most + per_group - 1) / per_group));
   if (plan.rows == kFewRows)
-    extend_join_kernel<T, D, kFewRows><<<grid, 256, 0, st>>>(a);
+    extend_join_kernel<T, D, kFewRows><<<grid, 256, 0, st>>>(a, lanes);
   else
-    extend_join_kernel<T, D, kTileRows><<<grid, 256, 0, st>>>(a);
+    extend_join_kernel<T, D, kTileRows><<<grid, 256, 0, st>>>(a, lanes);
 }
 
 template <typename T>
