@@ -123,9 +123,10 @@ __device__ __forceinline__ Place find_place(const Args& a, int tile) {
   return p;
 }
 
-// Pieces the tile's keys come in (at least one: empty rows are written too).
+// Pieces the tile's keys come in (at least one: empty rows are written too;
+// at most those the launch and the workspace have).
 __device__ __forceinline__ int parts_of(const Args& a, const Place& p) {
-  return a.parts == 1 ? 1 : max(1, (p.high - p.low + a.part_keys - 1) / a.part_keys);
+  return a.parts == 1 ? 1 : min(max(1, (p.high - p.low + a.part_keys - 1) / a.part_keys), a.parts);
 }
 
 // The keys a token sees are [low, high): those up to its own position or the

@@ -17,8 +17,13 @@
 // What a token does not see has no part in its row even where it is not
 // finite: a masked probability is 0, and a block in which some row masks a key
 // is multiplied key by key, skipping zeros, if its V holds a NaN or infinity
-// (0 times those would be NaN).  bfloat16 takes that way for every block with
-// such a V: an infinity times the second of the two values may be NaN.
+// (0 times those would be NaN).  bfloat16 does so for every block with such a
+// V: an infinity times the second of a probability's two values may be NaN.
+//
+// Bound by reading K and V where a sequence has one tile: 64 tokens over 512
+// to 8192 cached ones, 32 heads over 8 x 128 bfloat16, capped, 214 us (1145 MB
+// at 5.35 TB/s); one over 100000 75 us; 4 tokens at 2048, 12 x 64, 8.7 us, two
+// launches of dependent rounds.
 #include <limits.h>
 
 #include <algorithm>
@@ -418,9 +423,12 @@ __global__ __launch_bounds__(256) void extend_join_kernel(Args a, int lanes) {
 // (32 heads over 8 x 128, bfloat16) 240 with 2048 workgroups, 216 with 4096,
 // 216 with 8192, (12 x 64) 187, 155, 153; 1 x 2048 (12 x 64) 10.2 with
 // partitions of 256, 8.8 with 128, 13.5 with 512; 1 x 100000 76 with 256 and
-// 87 with 128 (many more to join).
+// 87 with 128 (many more to join).  Up to 256 keys stay in one piece: the join
+// costs more (1 and 8 tokens at 200, 12 x 64: 6.3 and 6.4 against 8.4 and 8.7;
+// at 400 9.5 against 8.7).
 constexpr int kGroups = 1024, kMinPart = 256;
 constexpr int kGroupsOnce = 4096, kMinPartOnce = 128;
+constexpr int kOnePiece = 256;
 
 struct Plan {
   int rows;  // of a tile
@@ -445,12 +453,14 @@ struct Plan {
 //   8 x 128: 1 x 256 + 0 (134) 25 / 43; 8 x 16 + 1000 (528) 66 / 51; 1 x 1000
 //   + 0 (2048) 193 / 137; 64 x 4 + 2000 (2099, 16 rows) 214 / 566.
 bool many_rows(int64_t tokens, int max_new, int64_t keys, int group, int kv_heads, int head_dim, int dtype) {
-  const int64_t work = tokens * group * kv_heads * (keys - std::min<int64_t>(max_new, keys) / 2) * head_dim;
-  if (dtype == MIE_DTYPE_F32) return static_cast<int64_t>(max_new) * group >= 64 && work >= 500'000'000;
-  return static_cast<int64_t>(max_new) * group > kFewRows && work >= 160'000'000;
+  const double work = static_cast<double>(tokens) * group * kv_heads * (keys - std::min<int64_t>(max_new, keys) / 2) *
+                      head_dim;
+  if (dtype == MIE_DTYPE_F32) return static_cast<int64_t>(max_new) * group >= 64 && work >= 500e6;
+  return static_cast<int64_t>(max_new) * group > kFewRows && work >= 160e6;
 }
 
 // Row tiles: as many as the batch can have (the lengths are on the device).
+// `window` is 0 where a prefix may be seen beyond it.
 // The keys are split until the tiles make the workgroups wanted.
 Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int group, int kv_heads, int head_dim,
                int dtype) {
@@ -468,7 +478,7 @@ Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int 
   const bool once = static_cast<int64_t>(max_new) * group <= kFewRows;
   const int min_part = once ? kMinPartOnce : kMinPart;
   const int64_t want = std::max<int64_t>(1, (once ? kGroupsOnce : kGroups) / (p.tiles * kv_heads));
-  const int64_t parts = std::min<int64_t>(want, (range + min_part - 1) / min_part);
+  const int64_t parts = range <= kOnePiece ? 1 : std::min<int64_t>(want, (range + min_part - 1) / min_part);
   if (parts <= 1) {
     p.parts = 1;
     p.part_keys = INT_MAX;
@@ -557,7 +567,8 @@ extern "C" int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q
   if (block_size < 1 || num_blocks < 1 || table_width < 1 || table_stride < table_width)
     return mie::fail(MIE_ERR_INVALID, "%s: block_size=%d num_blocks=%d table rows of %d, %lld apart", what, block_size,
                      num_blocks, table_width, static_cast<long long>(table_stride));
-  if (!(softcap >= 0.f) || !(softcap < INFINITY) || !(fabsf(scale) < INFINITY))
+  if (!(softcap >= 0.f) || !(softcap < INFINITY) || !(fabsf(scale * kLog2e) < INFINITY) ||
+      (softcap > 0.f && !(fabsf(2.f * kLog2e * scale / softcap) < INFINITY)))
     return mie::fail(MIE_ERR_INVALID, "%s: scale %g, softcap %g", what, scale, softcap);
   if (tokens == 0 || max_new == 0) return MIE_OK;
   if (!q || !k_pool || !v_pool || !starts || !context_lens || !out || !block_tables)
@@ -574,7 +585,8 @@ extern "C" int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q
     return mie::fail(MIE_ERR_INVALID, "%s: rows of q, out and the pools must be 16-byte aligned", what);
   max_new = std::min(max_new, tokens);
   const int group = num_heads / num_kv_heads;
-  const Plan plan = make_plan(tokens, batch, max_new, max_context_len, window, group, num_kv_heads, head_dim, dtype);
+  const Plan plan = make_plan(tokens, batch, max_new, max_context_len, prefix_lens ? 0 : window, group, num_kv_heads,
+                              head_dim, dtype);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return mie::fail(MIE_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", what,
                      static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));

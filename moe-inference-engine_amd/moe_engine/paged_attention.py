@@ -378,7 +378,8 @@ def extend_batched(
     Scores are scale * q . k (default 1 / sqrt(D)), then softcap * tanh(s /
     softcap) if softcap > 0, then - slopes[h] * |p - j| with slopes (float32
     [H]).  A token that sees no key gets 0.  Rows of q that no sequence has are
-    left as they are in `out` (uninitialised in a new tensor).
+    left as they are in `out` (uninitialised in a new tensor); a given out has
+    rows on 16-byte boundaries and is not q.
 
     float32 or bfloat16, D one of EXTEND_HEAD_DIMS; float32 sums and softmax.
     """
@@ -425,8 +426,8 @@ def extend_batched(
     _native.refuse_gradients("extend_batched", q, k_pool, v_pool, slopes)
     if out is None:
         out = torch.empty((tokens, heads, head_dim), dtype=dtype, device=device)
-    elif out.shape != q.shape or out.dtype != dtype or out.device != device:
-        raise ValueError(f"out must be {tuple(q.shape)} {dtype} on q's device")
+    elif out.shape != q.shape or out.dtype != dtype or out.device != device or out.stride(2) != 1:
+        raise ValueError(f"out must be {tuple(q.shape)} {dtype} on q's device with unit inner stride")
     elif out.data_ptr() == q.data_ptr() and tokens > 0:
         raise ValueError("out must not be q")
     if tokens == 0 or batch == 0:
@@ -437,8 +438,8 @@ def extend_batched(
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     lib, code = _native.lib(), _native.dtype_code(dtype)
-    nbytes = lib.mie_paged_extend_workspace(tokens, batch, max_new_tokens, max_context_len, window, heads, kv_heads,
-                                            head_dim, code)
+    nbytes = lib.mie_paged_extend_workspace(tokens, batch, max_new_tokens, max_context_len,
+                                            0 if prefix_lens is not None else window, heads, kv_heads, head_dim, code)
     if nbytes < 0:
         _native.check(-nbytes, "mie_paged_extend_workspace")
     ws = _workspace(nbytes, device)

@@ -237,6 +237,20 @@ def test_scores_and_masks_of_many_rows(option, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_a_prefix_far_past_the_window_over_a_split_context(dtype):
+    """The prefix's keys count for the split, not the window's alone."""
+    print_case("extend prefix past window", dtype)
+    for new, old, heads in (([2, 1], [300, 9000], 2), ([150, 40], [600, 9000], 8)):
+        c = batch(new, old, heads, 1, 64, 16, dtype, seed=3, heavy=0.01)
+        for prefix in (list(c["len_list"]), [n // 2 for n in c["len_list"]]):
+            kw = dict(window=64, prefix_lens=torch.tensor(prefix, dtype=torch.int32, device=DEV))
+            check(c, call(c, max_len=9150, **kw), window=64, prefix=prefix)
+    # All of a long sequence is new: its first tokens see the whole prefix, far past the window.
+    c = batch([1500], [0], 2, 1, 64, 16, dtype, seed=5)
+    check(c, call(c, window=16, prefix_lens=torch.tensor([1400], dtype=torch.int32, device=DEV)), window=16, prefix=[1400])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_many_rows_over_a_split_context(dtype):
     print_case("extend many rows split", dtype)
     c = batch([150, 40], [6000, 2500], 8, 1, 64, 16, dtype, seed=3, heavy=0.01)

@@ -30,6 +30,8 @@ def test_score_on_the_gpu_is_the_cpus(paged):
     for g, w in zip(got[:3], want[:3]):
         assert g.is_cuda and float((g.cpu() - w).abs().max()) < 500 * 10 * 2.0**-24
     assert projection.token_logprobs(torch.zeros(1, 5, device=DEV)).logprobs is None
+    one = model.score(ids[:1].to(DEV), top=2)
+    assert one.logprobs.shape == (0,) and one.top_tokens.shape == (0, 2)
 
 
 class Layer:

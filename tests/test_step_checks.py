@@ -92,6 +92,8 @@ CASES = [
     ("mie_paged_extend", extend_args(cap=math.inf), INVALID, b"softcap"),
     ("mie_paged_extend", extend_args(cap=math.nan), INVALID, b"softcap"),
     ("mie_paged_extend", extend_args(scale=math.nan), INVALID, b"scale"),
+    ("mie_paged_extend", extend_args(scale=3e38), INVALID, b"scale"),
+    ("mie_paged_extend", extend_args(cap=1e-40), INVALID, b"softcap"),
     ("mie_paged_extend", extend_args(t_stride=9), INVALID, b"table rows"),
     ("mie_paged_extend", extend_args(block_size=0), INVALID, b"block_size=0"),
     ("mie_paged_extend", extend_args(starts=None), INVALID, b"null pointer"),
@@ -230,6 +232,8 @@ EXTEND = dict(q=torch.zeros(3, 4, 64), k_pool=torch.zeros(1, 5, 2, 4, 64), v_poo
     (dict(window=-1), ValueError, "window"), (dict(softcap=-1.0), ValueError, "softcap"),
     (dict(softcap=math.nan), ValueError, "softcap"), (dict(out=torch.zeros(3, 4, 32)), ValueError, "out must be"),
     (dict(out=EXTEND["q"]), ValueError, "out must not be q"),
+    (dict(out=torch.zeros(3, 64, 4).transpose(1, 2)), ValueError, "unit inner stride"),
+    (dict(block_tables=torch.zeros(2, 0, dtype=torch.int32)), ValueError, "block tables"),
     (dict(q=torch.zeros(3, 4, 64, requires_grad=True)), RuntimeError, "backward"),
 ], ids=str)
 def test_extend_batched_refuses(device, change, error, message):
