@@ -12,7 +12,10 @@
 // of the tokens; workgroup 0 also writes what there is one of per sequence.
 // Nothing that is read is written in the same launch: the table entries
 // written are those of blocks the step takes, the entries read those of blocks
-// held before, and the counts and lengths go to other arrays.
+// held before, and the counts and lengths go to other arrays.  Bound by
+// latency (three dependent rounds and two scans): on MI355X 4.5 us for a decode
+// step of 64 sequences, 10.6 us for a million tokens of 500 (13 MB, 2.6 us at
+// the rate of a copy), 7.2 us for the release of 1000 sequences' 250 000 blocks.
 #include <limits.h>
 
 #include <algorithm>
