@@ -95,9 +95,10 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   const float m = fmaxf(a.m, b.m);
   auto shift = [&](Sums& x) {
     const float d = x.m - m, f = mie::fast_exp2(d * kLog2e);
-    // A part without weight has nothing to shift (its distance may be infinite).
-    x.e = x.s == 0.f ? 0.f : (x.e + x.s * d) * f;
-    x.s = x.s == 0.f ? 0.f : x.s * f;
+    // What is out of reach is dropped: sums of float32's lowest values would
+    // overflow on the way to 0.
+    x.e = f == 0.f ? 0.f : (x.e + x.s * d) * f;
+    x.s = f == 0.f ? 0.f : x.s * f;
   };
   shift(a);
   shift(b);
@@ -281,8 +282,8 @@ __global__ __launch_bounds__(kThreads, 4) void token_logprobs_kernel(LogprobsArg
       const float to = fmaxf(top, m), d = m - to, f = mie::fast_exp2(d * kLog2e);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        e[j] = s[j] == 0.f ? 0.f : (e[j] + s[j] * d) * f;
-        s[j] = s[j] == 0.f ? 0.f : s[j] * f;
+        e[j] = f == 0.f ? 0.f : (e[j] + s[j] * d) * f;  // as in join
+        s[j] = f == 0.f ? 0.f : s[j] * f;
       }
       m = to;
     }

@@ -100,6 +100,21 @@ def test_large_values():
     assert bool(torch.isfinite(got.entropy).all()) and float(got.entropy[1]) == 0
 
 
+@pytest.mark.parametrize("where", ["most", "front", "behind"])
+@pytest.mark.parametrize("rows,vocab", [(1, 300), (3, 50257), (2, 150000), (600, 5000)])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_tokens_masked_by_the_types_lowest_value(where, rows, vocab, dtype):
+    print_case("logprobs lowest", where, rows, vocab, dtype)
+    g = torch.Generator().manual_seed(vocab)
+    i = torch.arange(vocab)
+    masked = {"most": torch.rand(vocab, generator=g) < 0.99, "front": i < vocab - 20, "behind": i >= 20}[where]
+    masked[123] = False
+    x = torch.randn(rows, vocab, generator=g).to(dtype).masked_fill(masked, torch.finfo(dtype).min).to(DEV)
+    tokens = torch.arange(rows).clamp(max=200)
+    tokens[::2] = 123
+    check(x, tokens.to(DEV), 20)
+
+
 @pytest.mark.parametrize("vocab", [50, 3000, 50257, 150000])
 def test_values_that_are_not_finite(vocab):
     print_case("logprobs nan", vocab)
