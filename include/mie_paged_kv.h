@@ -785,7 +785,8 @@ int32_t mie_token_logprobs(const void* logits, int64_t stride, int32_t rows, int
  *   (j <= p, or j < prefix_lens[b] if prefix_lens is non-NULL)
  *   and (j > p - window, if window > 0),
  * and for head h, reading K/V head h / (num_heads / num_kv_heads):
- *   s_j = scale * q . k_j;  s_j = softcap * tanh(s_j / softcap) if softcap > 0;
+ *   s_j = scale * q . k_j;  s_j = softcap * tanh(s_j / softcap) if softcap > 0
+ *   (at most 1024);
  *   s_j -= slopes[h] * |p - j| if slopes (float32 [num_heads]) is non-NULL;
  *   out = sum_j softmax(s)_j v_j       (0 for a token that sees no key)
  * with sums, maxima and softmax in float32 and the output rounded once.  Keys

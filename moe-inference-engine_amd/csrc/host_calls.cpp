@@ -265,11 +265,11 @@ const int32_t* ints(const at::Tensor* t) { return t ? static_cast<const int32_t*
 int32_t* ints_out(const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
 
 // Block tables [B, n]: rows of int32, not overlapping.
-const at::Tensor* table_rows(PyObject* o, c10::Device device, bool distinct) {
+const at::Tensor* table_rows(PyObject* o, c10::Device device) {
   const at::Tensor* t = plain(o);
   if (!t || t->dim() != 2 || t->scalar_type() != at::kInt || t->device() != device || t->size(0) < 1 ||
       t->size(1) < 1 || t->stride(1) != 1 || !fits(t->size(0)) || !fits(t->size(1)) ||
-      (distinct && t->size(0) > 1 && t->stride(0) < t->size(1)))
+      (t->size(0) > 1 && t->stride(0) < t->size(1)))
     return nullptr;
   return t;
 }
@@ -283,7 +283,7 @@ PyObject* reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int64_t block, tokens, stream;
   if (!ids || !as_int(a[5], block) || !as_int(a[6], tokens) || !as_int(a[7], stream)) Py_RETURN_NONE;
   const auto device = ids->device();
-  const at::Tensor* tables = table_rows(a[2], device, true);
+  const at::Tensor* tables = table_rows(a[2], device);
   if (!tables || !vec(a[0], at::kInt, device, -1)) Py_RETURN_NONE;
   const int64_t batch = tables->size(0);
   const at::Tensor *count = vec(a[1], at::kInt, device, 1), *lens = vec(a[3], at::kInt, device, batch),
@@ -316,7 +316,7 @@ PyObject* release(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int64_t block, stream;
   if (!ids || !as_int(a[5], block) || !as_int(a[6], stream)) Py_RETURN_NONE;
   const auto device = ids->device();
-  const at::Tensor* tables = table_rows(a[2], device, true);
+  const at::Tensor* tables = table_rows(a[2], device);
   if (!tables || !vec(a[0], at::kInt, device, -1)) Py_RETURN_NONE;
   const int64_t batch = tables->size(0);
   const at::Tensor *count = vec(a[1], at::kInt, device, 1), *lens = vec(a[3], at::kInt, device, batch),
@@ -400,7 +400,7 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const auto ps = kp->sizes();
   const int64_t tokens = q->size(0), heads = q->size(1), blocks = ps[1], kv_heads = ps[2], block = ps[3], dim = ps[4];
   const int64_t align = 16 / q->element_size();
-  const at::Tensor* tables = table_rows(a[4], device, false);
+  const at::Tensor* tables = table_rows(a[4], device);
   if (!tables || tokens < 1 || q->size(2) != dim || q->stride(2) != 1 || q->stride(0) % align ||
       q->stride(1) % align || reinterpret_cast<uintptr_t>(q->data_ptr()) % 16 || layer < 0 || layer >= ps[0] ||
       kv_heads < 1 || heads < 1 || heads % kv_heads || !fits(tokens) || !fits(heads) || !fits(blocks) || !fits(block) ||

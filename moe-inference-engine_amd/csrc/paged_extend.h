@@ -19,6 +19,7 @@ using gemm::f32x4;
 using gemm::u32x4;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMaxSoftcap = 1024.f;
 constexpr int kFewRows = 16;    // rows per workgroup where a sequence has few (extend_rows_kernel)
 constexpr int kTileRows = 128;  // and where it has many (extend_tile_kernel)
 
@@ -148,8 +149,8 @@ __device__ __forceinline__ bool holds(Range r, int key) {
 
 // cap tanh(q . k scale / softcap) in base 2 (Args: cap, scale, cap_ratio).
 // tanh(x) = 1 - 2 / (exp(2 x) + 1) has an absolute error of 2^-23, times the
-// cap a few 1e-6 of the exponent, which bfloat16 does not show; float32 takes
-// the library's.
+// cap a few 1e-6 of the exponent (at most 4e-4, kMaxSoftcap), which bfloat16
+// does not show; float32 takes the library's.
 template <typename T>
 __device__ __forceinline__ float capped(float dot, float cap, float scale, float ratio) {
   if constexpr (sizeof(T) == 4) return cap * tanhf(dot * ratio);

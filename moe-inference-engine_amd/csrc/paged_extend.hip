@@ -567,7 +567,8 @@ extern "C" int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q
   if (block_size < 1 || num_blocks < 1 || table_width < 1 || table_stride < table_width)
     return mie::fail(MIE_ERR_INVALID, "%s: block_size=%d num_blocks=%d table rows of %d, %lld apart", what, block_size,
                      num_blocks, table_width, static_cast<long long>(table_stride));
-  if (!(softcap >= 0.f) || !(softcap < INFINITY) || !(fabsf(scale * kLog2e) < INFINITY) ||
+  // A larger cap would show what tanh leaves of small scores in float32.
+  if (!(softcap >= 0.f) || !(softcap <= mie::extend::kMaxSoftcap) || !(fabsf(scale * kLog2e) < INFINITY) ||
       (softcap > 0.f && !(fabsf(2.f * kLog2e * scale / softcap) < INFINITY)))
     return mie::fail(MIE_ERR_INVALID, "%s: scale %g, softcap %g", what, scale, softcap);
   if (tokens == 0 || max_new == 0) return MIE_OK;
@@ -619,7 +620,7 @@ extern "C" int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q
   a.cap = softcap * kLog2e;
   a.cap_ratio = softcap > 0.f ? scale / softcap : 0.f;
   a.slopes = slopes;
-  a.window = window;
+  a.window = window > 1 << 30 ? 0 : window;  // no length reaches farther; positions less the window stay in 31 bits
   a.prefix = prefix_lens;
   a.whole_blocks = block_size % 16 == 0;
   a.tiles = static_cast<int32_t>(plan.tiles);

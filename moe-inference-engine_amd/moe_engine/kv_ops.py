@@ -291,8 +291,8 @@ def _check_step(free_ids, free_count, block_tables, context_lens, block_size):
                        ("context_lens", context_lens, batch)):
         if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or t.device != device or not t.is_contiguous():
             raise ValueError(f"{name} must be {n} contiguous int32 values on the free list's device")
-    if int(block_size) < 1:
-        raise ValueError(f"block_size {block_size}")
+    if not 1 <= int(block_size) < 1 << 31 or free_ids.numel() > 1 << 30:
+        raise ValueError(f"block_size {block_size}, {free_ids.numel()} free ids (at most 2^30)")
     return batch, device
 
 
@@ -335,8 +335,8 @@ def reserve(
             or not new_lens.is_contiguous():
         raise ValueError(f"new_lens must be {batch} contiguous int32 values on the free list's device")
     max_tokens = int(max_tokens)
-    if max_tokens < 0:
-        raise ValueError(f"max_tokens {max_tokens}")
+    if not 0 <= max_tokens <= 1 << 30:
+        raise ValueError(f"max_tokens {max_tokens} outside [0, 2^30]")
     word = dict(dtype=torch.int32, device=device)
     starts, positions = torch.empty(batch + 1, **word), torch.empty(max_tokens, **word)
     slots = torch.empty(max_tokens, dtype=torch.int64, device=device)

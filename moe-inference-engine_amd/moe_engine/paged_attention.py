@@ -376,7 +376,7 @@ def extend_batched(
     A token at position p sees the keys j <= p of its sequence; with prefix_lens
     (int32 [B]) also all j < prefix_lens[b]; with window > 0 only j > p - window.
     Scores are scale * q . k (default 1 / sqrt(D)), then softcap * tanh(s /
-    softcap) if softcap > 0, then - slopes[h] * |p - j| with slopes (float32
+    softcap) if softcap > 0 (at most 1024), then - slopes[h] * |p - j| with slopes (float32
     [H]).  A token that sees no key gets 0.  Rows of q that no sequence has are
     left as they are in `out` (uninitialised in a new tensor); a given out has
     rows on 16-byte boundaries and is not q.
@@ -421,8 +421,12 @@ def extend_batched(
     max_new_tokens, max_context_len, window = int(max_new_tokens), int(max_context_len), int(window)
     if max_new_tokens < 0 or max_context_len < 0 or window < 0:
         raise ValueError("max_new_tokens, max_context_len and window must not be negative")
-    if not (0 <= softcap < math.inf):
-        raise ValueError(f"softcap {softcap} must be finite and not negative (0: none)")
+    if max_context_len > 1 << 30:
+        raise ValueError(f"max_context_len {max_context_len} above 2^30")
+    # What a bound beyond every length means, in the 32 bits of the call.
+    max_new_tokens, window = min(max_new_tokens, tokens), 0 if window > 1 << 30 else window
+    if not (0 <= softcap <= 1024):
+        raise ValueError(f"softcap {softcap} outside [0, 1024] (0: none)")
     _native.refuse_gradients("extend_batched", q, k_pool, v_pool, slopes)
     if out is None:
         out = torch.empty((tokens, heads, head_dim), dtype=dtype, device=device)
@@ -432,6 +436,8 @@ def extend_batched(
         raise ValueError("out must not be q")
     if tokens == 0 or batch == 0:
         return out
+    if batch > 1 and block_tables.stride(0) < block_tables.shape[1]:  # rows that overlap, one for all for instance
+        block_tables = block_tables.contiguous()
     align = 16 // q.element_size()
     if q.stride(2) != 1 or q.stride(0) % align or q.stride(1) % align or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)

@@ -251,6 +251,8 @@ def token_logprobs(logits, tokens=None, top: int = 0) -> TokenLogprobs:
     if not _native.is_rocm_device(logits):
         raise RuntimeError("mie_token_logprobs needs tensors on a ROCm device")
     rows, vocab = logits.shape
+    if rows > 1 << 20 or vocab > 1 << 30:
+        raise ValueError(f"{rows} rows (at most 2^20) of {vocab} (2^30)")
     if tokens is not None and (tokens.dtype != torch.int64 or tokens.shape != (rows,)
                                or tokens.device != logits.device):
         raise ValueError(f"tokens must be {rows} int64 values on the logits' device")

@@ -381,6 +381,40 @@ def test_strides(how):
         assert bool((out._base[:, 0] == 0).all() and (out._base[:, 5] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_the_largest_bounds(dtype):
+    """Bounds beyond every length, in 32 bits and past them, mean no bound; a
+    length below the new tokens puts the first ones before position 0."""
+    print_case("extend largest bounds", dtype)
+    c = batch([1, 40, 150], [400, 3, 90], 4, 2, 64, 16, dtype, seed=7)
+    for window, most in ((2**30, 2**31 - 1), (2**30 + 1, 2**31), (2**31 - 1, 2**32), (2**32, 2**33)):
+        check(c, call(c, max_new=most, window=window))
+    check(c, call(c, max_len=2**30))
+    check(c, call(c, softcap=1024.0, scale=1.0), softcap=1024.0, scale=1.0)
+    # 40 new tokens of a length of 30: the first see the prefix alone.
+    c["len_list"][1], c["lens"][1] = 30, 30
+    c["keys"][1] = tuple(t[:30] for t in c["keys"][1])
+    prefix = torch.tensor([0, 20, 0], dtype=torch.int32, device=DEV)
+    for window in (0, 2**31 - 1):
+        check(c, call(c, window=window, prefix_lens=prefix), prefix=[0, 20, 0])
+
+
+@pytest.mark.parametrize("to_out", [False, True])
+def test_one_table_row_for_every_sequence(to_out):
+    """A broadcast table, and rows that overlap: the same as their copies."""
+    print_case("extend shared table", to_out)
+    c = batch([1], [200], 4, 2, 64, 16, BF16, seed=11)
+    q = torch.randn(5, 4, 64, device=DEV).to(BF16)
+    starts = torch.arange(6, dtype=torch.int32, device=DEV)
+    lens = torch.tensor([201, 3, 90, 64, 17], dtype=torch.int32, device=DEV)
+    line = torch.cat([c["tables"][0], c["tables"][0, :4]])
+    for tables in (c["tables"].expand(5, -1), line.as_strided((5, 13), (1, 1))):
+        got, want = (paged_attention.extend_batched(
+            q, c["k"], c["v"], 1, t, starts, lens, 1, 201, out=torch.empty_like(q) if to_out else None)
+            for t in (tables, tables.contiguous()))
+        assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0)) and not bool(got[0].isnan().any())
+
+
 def test_it_is_decode_where_each_sequence_has_one_token():
     print_case("extend vs decode")
     c = batch([1] * 5, [0, 30, 500, 1000, 2500], 4, 4, 64, 16, F32, seed=9)

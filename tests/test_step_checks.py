@@ -90,6 +90,7 @@ CASES = [
     ("mie_paged_extend", extend_args(max_len=-1), INVALID, b"max_context_len=-1"),
     ("mie_paged_extend", extend_args(cap=-1.0), INVALID, b"softcap"),
     ("mie_paged_extend", extend_args(cap=math.inf), INVALID, b"softcap"),
+    ("mie_paged_extend", extend_args(cap=1025.0), INVALID, b"softcap"),
     ("mie_paged_extend", extend_args(cap=math.nan), INVALID, b"softcap"),
     ("mie_paged_extend", extend_args(scale=math.nan), INVALID, b"scale"),
     ("mie_paged_extend", extend_args(scale=3e38), INVALID, b"scale"),
@@ -231,7 +232,8 @@ EXTEND = dict(q=torch.zeros(3, 4, 64), k_pool=torch.zeros(1, 5, 2, 4, 64), v_poo
     (dict(slopes=torch.zeros(2)), ValueError, "slopes"), (dict(slopes=torch.zeros(4).double()), ValueError, "slopes"),
     (dict(window=-1), ValueError, "window"), (dict(softcap=-1.0), ValueError, "softcap"),
     (dict(softcap=math.nan), ValueError, "softcap"), (dict(out=torch.zeros(3, 4, 32)), ValueError, "out must be"),
-    (dict(out=EXTEND["q"]), ValueError, "out must not be q"),
+    (dict(out=EXTEND["q"]), ValueError, "out must not be q"), (dict(softcap=1025), ValueError, "softcap"),
+    (dict(max_context_len=2**32 + 5), ValueError, "max_context_len"),
     (dict(out=torch.zeros(3, 64, 4).transpose(1, 2)), ValueError, "unit inner stride"),
     (dict(block_tables=torch.zeros(2, 0, dtype=torch.int32)), ValueError, "block tables"),
     (dict(q=torch.zeros(3, 4, 64, requires_grad=True)), RuntimeError, "backward"),
