@@ -112,3 +112,34 @@ def test_same_refusals(monkeypatch):
                 call()
     with torch.no_grad():
         projection.token_logprobs(q.detach()[0].requires_grad_(), slots)
+
+
+@pytest.mark.gpu
+def test_in_inference_mode_and_on_another_stream(monkeypatch):
+    """A step under inference mode, each call on a stream of its own."""
+    print_case("step host calls, inference mode")
+    ids, count = torch.arange(50, device=DEV).int(), torch.tensor([50], dtype=torch.int32, device=DEV)
+    tables, lens = torch.zeros(2, 8, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+    new = torch.tensor([30, 9], dtype=torch.int32, device=DEV)
+    freq, _ = kv_ops.rope_frequencies(64, device=DEV)
+    pools = [torch.zeros(1, 50, 2, 8, 64, device=DEV) for _ in range(4)]
+    qkv = torch.randn(40, 8, 64, device=DEV)
+    q, k, v = qkv.split([4, 2, 2], 1)
+
+    def step(kp, vp):
+        r = kv_ops.reserve(ids, count, tables, lens, new, 8, 40)
+        x = kv_ops.rope_append(q, k, v, kp, vp, 0, r.slots, r.positions, freq)
+        y = paged_attention.extend_batched(x, kp, vp, 0, tables, r.starts, r.context_lens, 30, 30)[:39]
+        p = projection.token_logprobs(y.reshape(39, 256), torch.arange(39, device=DEV), top=3)
+        done = kv_ops.release(ids.clone(), r.free_count, tables, r.context_lens, new > 10, 8)
+        return [*r, x, y, *p, *done]
+
+    want = step(*pools[:2])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.inference_mode(), torch.cuda.stream(stream):
+        got = step(*pools[2:])
+        assert all(t.is_inference() for t in got if t is not None)
+        got[0].add_(0)  # a piece of a shared allocation is a tensor like another
+    torch.cuda.current_stream().wait_stream(stream)
+    assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
