@@ -800,9 +800,8 @@ int32_t mie_token_logprobs(const void* logits, int64_t stride, int32_t rows, int
  * bfloat16; num_heads / num_kv_heads whole and at most 128; tokens <= 2^22.
  *
  * One launch, or two where the context is split: the workspace is
- * mie_paged_extend_workspace's bytes for the same arguments, but with window 0
- * where prefix_lens is given (negative: -MIE_ERR_*), and nothing in it needs
- * clearing.
+ * mie_paged_extend_workspace's bytes for the same arguments (negative:
+ * -MIE_ERR_*), and nothing in it needs clearing.
  */
 int64_t mie_paged_extend_workspace(int32_t tokens, int32_t batch, int32_t max_new, int32_t max_context_len,
                                    int32_t window, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,

@@ -413,8 +413,7 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       (a[13] != Py_None && !(prefix = vec(a[13], at::kInt, device, batch))) || !usual({q, kp, vp, slopes}))
     Py_RETURN_NONE;
   if (a[9] == Py_None) scale = 1.0 / std::sqrt(static_cast<double>(dim));
-  const int64_t bytes =
-      g_extend_workspace(tokens, batch, max_new, max_len, prefix ? 0 : window, heads, kv_heads, dim, code);
+  const int64_t bytes = g_extend_workspace(tokens, batch, max_new, max_len, window, heads, kv_heads, dim, code);
   if (bytes < 0) Py_RETURN_NONE;  // refused: the other path says why
   at::Tensor out = at::empty({tokens, heads, dim}, q->options().requires_grad(false)), ws;
   if (bytes > 0) ws = at::empty({bytes}, q->options().dtype(at::kByte).requires_grad(false));

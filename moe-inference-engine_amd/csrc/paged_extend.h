@@ -7,6 +7,7 @@
 // that is read.
 #pragma once
 
+#include <limits.h>
 #include <math.h>
 
 #include "gemm_tile.h"
@@ -43,7 +44,7 @@ struct Args {
   int32_t window;
   const int32_t* prefix;
   int32_t tiles;             // row tiles of the launch, a bound
-  int32_t parts, part_keys;  // a row tile's keys in `parts` pieces of part_keys at most
+  int32_t parts, part_keys;  // a row tile's keys in at most `parts` pieces, of part_keys or more
   float* ws_acc;             // [tile, kv head, part, row, D]
   float* ws_ml;              // [tile, kv head, part, row, 2]
   int32_t whole_blocks;      // blocks hold a multiple of 16 keys
@@ -124,10 +125,33 @@ __device__ __forceinline__ Place find_place(const Args& a, int tile) {
   return p;
 }
 
-// Pieces the tile's keys come in (at least one: empty rows are written too;
-// at most those the launch and the workspace have).
-__device__ __forceinline__ int parts_of(const Args& a, const Place& p) {
-  return a.parts == 1 ? 1 : min(max(1, (p.high - p.low + a.part_keys - 1) / a.part_keys), a.parts);
+// A workgroup's K/V head, row tile and part: heads side by side, then tiles,
+// all first parts before the second ones.  Workgroups go to the XCDs and their
+// shader engines in turn, and a short tile's later parts are empty: with a
+// tile's parts side by side the engines at the places of the later ones had
+// less to do (8 chunks of 100 to 500 float32 tokens behind 1000 to 4000 in two
+// parts 1810 us, 945 this way; 64 decode tokens 222 and 212).  For the same
+// reason the tiles of each part start one later.
+struct Item {
+  int kvh, tile, part;
+};
+__device__ __forceinline__ Item item_of(const Args& a) {
+  const int kvh = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
+  const int part = item / a.tiles;
+  return Item{kvh, (item + part) % a.tiles, part};
+}
+
+// Pieces the tile's keys come in: at least one (empty rows are written too), at
+// most those the launch and the workspace have, each larger where these do not
+// hold the keys (a prefix may end far beyond the window the host counted).
+struct Split {
+  int parts, keys;
+};
+__device__ __forceinline__ Split split_of(const Args& a, const Place& p) {
+  if (a.parts == 1) return Split{1, INT_MAX};
+  const int range = p.high - p.low;
+  const int keys = max(a.part_keys, ((range + a.parts - 1) / a.parts + 127) & ~127);
+  return Split{max(1, (range + keys - 1) / keys), keys};
 }
 
 // The keys a token sees are [low, high): those up to its own position or the

@@ -148,14 +148,15 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_rows
   __shared__ __align__(16) int64_t s_off[4][2][32];  // each wave's row offsets, this block's and the next one's
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kvh = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
-  const int part = item % a.parts, tile = item / a.parts;
+  const mie::extend::Item item = mie::extend::item_of(a);
+  const int kvh = item.kvh, part = item.part, tile = item.tile;
   const Place p = mie::extend::find_place<kRows>(a, tile);
   if (p.b < 0) return;
-  const int parts = mie::extend::parts_of(a, p);
+  const mie::extend::Split split = mie::extend::split_of(a, p);
+  const int parts = split.parts;
   if (part >= parts) return;
-  const int first = p.low + part * a.part_keys;
-  const int end = parts == 1 ? p.high : min(p.high, first + a.part_keys);
+  const int first = p.low + part * split.keys;
+  const int end = parts == 1 ? p.high : min(p.high, first + split.keys);
 
   // This lane's row (the last one again past the end), its head and position.
   const int row = min(p.row0 + i, p.rows - 1);
@@ -373,7 +374,7 @@ __global__ __launch_bounds__(256) void extend_join_kernel(Args a, int lanes) {
   const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
   const Place p = mie::extend::find_place<ROWS>(a, tile);
   if (p.b < 0) return;
-  const int parts = mie::extend::parts_of(a, p);
+  const int parts = mie::extend::split_of(a, p).parts;
   if (parts == 1) return;
   const int col = threadIdx.x % kCols, at = threadIdx.x / kCols;
   const int lane = at & (lanes - 1), in_tile = blockIdx.y * (kAtOnce / lanes) + at / lanes;
@@ -417,17 +418,25 @@ __global__ __launch_bounds__(256) void extend_join_kernel(Args a, int lanes) {
 // ---- host ------------------------------------------------------------------
 
 // Workgroups that the keys are split for, and the keys of the smallest
-// partition: in general, and where a sequence has one tile, so that its keys
+// partition: of 16 rows; where a sequence has one such tile, so that its keys
 // are read once and reading them is the work (its partitions also even out
-// ragged lengths).  Measured on MI355X, us: 64 sequences of 512 to 8192 tokens
-// (32 heads over 8 x 128, bfloat16) 240 with 2048 workgroups, 216 with 4096,
-// 216 with 8192, (12 x 64) 187, 155, 153; 1 x 2048 (12 x 64) 10.2 with
-// partitions of 256, 8.8 with 128, 13.5 with 512; 1 x 100000 76 with 256 and
-// 87 with 128 (many more to join).  Up to 256 keys stay in one piece: the join
+// ragged lengths); of 128 rows in float32 and in bfloat16 (whose products take
+// an eighth of the time, so that partitions and their join weigh more).
+// Measured on MI355X, us, once: 64 sequences of 512 to 8192 tokens (32 heads
+// over 8 x 128, bfloat16) 210 with 2048 workgroups, 212 with 4096, 228 with
+// 8192, (12 x 64) 175, 156, 152; 1 x 2048 (12 x 64) 10.2 with partitions of
+// 256, 8.8 with 128, 13.5 with 512; 1 x 100000 76 with 256 and 87 with 128
+// (many more to join).  128 rows, bfloat16: 512 + 1500 (12 x 64) 23.3 with 1024
+// workgroups of 256 keys, 20.5 with 512 of 384; 1000 + 0 21.5, 18.5; two of 512
+// + 3500 (32 over 8 x 128) 114, 98; four of 50 to 300 + up to 8000 63, 57.
+// float32: 512 + 1500 (12 x 64) 53 with 256 keys, 51 with 128; six of up to 700
+// + 1300 (8 x 96) 80 with 1024 workgroups, 102 with 2048.  Up to 256 keys stay in one piece: the join
 // costs more (1 and 8 tokens at 200, 12 x 64: 6.3 and 6.4 against 8.4 and 8.7;
 // at 400 9.5 against 8.7).
 constexpr int kGroups = 1024, kMinPart = 256;
 constexpr int kGroupsOnce = 4096, kMinPartOnce = 128;
+constexpr int kGroupsTileF32 = 1024, kMinPartTileF32 = 128;
+constexpr int kGroupsTile = 512, kMinPartTile = 384;
 constexpr int kOnePiece = 256;
 
 struct Plan {
@@ -460,7 +469,6 @@ bool many_rows(int64_t tokens, int max_new, int64_t keys, int group, int kv_head
 }
 
 // Row tiles: as many as the batch can have (the lengths are on the device).
-// `window` is 0 where a prefix may be seen beyond it.
 // The keys are split until the tiles make the workgroups wanted.
 Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int group, int kv_heads, int head_dim,
                int dtype) {
@@ -476,8 +484,12 @@ Plan make_plan(int tokens, int batch, int max_new, int max_len, int window, int 
   const int64_t span = (rows + group - 1) / group + 1;
   const int64_t range = window > 0 ? std::min<int64_t>(max_len, static_cast<int64_t>(window) + span + 32) : max_len;
   const bool once = static_cast<int64_t>(max_new) * group <= kFewRows;
-  const int min_part = once ? kMinPartOnce : kMinPart;
-  const int64_t want = std::max<int64_t>(1, (once ? kGroupsOnce : kGroups) / (p.tiles * kv_heads));
+  int groups = once ? kGroupsOnce : kGroups, min_part = once ? kMinPartOnce : kMinPart;
+  if (rows == kTileRows) {
+    groups = dtype == MIE_DTYPE_F32 ? kGroupsTileF32 : kGroupsTile;
+    min_part = dtype == MIE_DTYPE_F32 ? kMinPartTileF32 : kMinPartTile;
+  }
+  const int64_t want = std::max<int64_t>(1, groups / (p.tiles * kv_heads));
   const int64_t parts = range <= kOnePiece ? 1 : std::min<int64_t>(want, (range + min_part - 1) / min_part);
   if (parts <= 1) {
     p.parts = 1;
@@ -586,8 +598,7 @@ extern "C" int32_t mie_paged_extend(const void* q, int64_t q_stride_t, int64_t q
     return mie::fail(MIE_ERR_INVALID, "%s: rows of q, out and the pools must be 16-byte aligned", what);
   max_new = std::min(max_new, tokens);
   const int group = num_heads / num_kv_heads;
-  const Plan plan = make_plan(tokens, batch, max_new, max_context_len, prefix_lens ? 0 : window, group, num_kv_heads,
-                              head_dim, dtype);
+  const Plan plan = make_plan(tokens, batch, max_new, max_context_len, window, group, num_kv_heads, head_dim, dtype);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return mie::fail(MIE_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)", what,
                      static_cast<long long>(workspace_bytes), static_cast<long long>(plan.bytes));

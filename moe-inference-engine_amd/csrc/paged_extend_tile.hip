@@ -343,14 +343,15 @@ __global__ __launch_bounds__(256, D * sizeof(T) <= 384 ? 2 : 1) void extend_tile
   __shared__ int s_bad, s_odd;  // a key without a block; a dropped value
   const int lane = threadIdx.x & 63, q = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kvh = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
-  const int part = item % a.parts, tile = a.tiles - 1 - item / a.parts;
+  const mie::extend::Item item = mie::extend::item_of(a);
+  const int kvh = item.kvh, part = item.part, tile = a.tiles - 1 - item.tile;
   const Place p = mie::extend::find_place<kTileRows>(a, tile);
   if (p.b < 0) return;
-  const int parts = mie::extend::parts_of(a, p);
+  const mie::extend::Split split = mie::extend::split_of(a, p);
+  const int parts = split.parts;
   if (part >= parts) return;
-  const int first = p.low + part * a.part_keys;
-  const int end = parts == 1 ? p.high : min(p.high, first + a.part_keys);
+  const int first = p.low + part * split.keys;
+  const int end = parts == 1 ? p.high : min(p.high, first + split.keys);
   if (threadIdx.x == 0) s_bad = s_odd = 0;
 
   State<T, D> w;

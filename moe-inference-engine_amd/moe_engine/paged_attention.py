@@ -444,8 +444,8 @@ def extend_batched(
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     lib, code = _native.lib(), _native.dtype_code(dtype)
-    nbytes = lib.mie_paged_extend_workspace(tokens, batch, max_new_tokens, max_context_len,
-                                            0 if prefix_lens is not None else window, heads, kv_heads, head_dim, code)
+    nbytes = lib.mie_paged_extend_workspace(tokens, batch, max_new_tokens, max_context_len, window, heads, kv_heads,
+                                            head_dim, code)
     if nbytes < 0:
         _native.check(-nbytes, "mie_paged_extend_workspace")
     ws = _workspace(nbytes, device)
