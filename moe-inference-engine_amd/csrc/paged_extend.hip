@@ -21,8 +21,8 @@
 // V: an infinity times the second of a probability's two values may be NaN.
 //
 // Bound by reading K and V where a sequence has one tile: 64 tokens over 512
-// to 8192 cached ones, 32 heads over 8 x 128 bfloat16, capped, 214 us (1145 MB
-// at 5.35 TB/s); one over 100000 75 us; 4 tokens at 2048, 12 x 64, 8.7 us, two
+// to 8192 cached ones, 32 heads over 8 x 128 bfloat16, capped, 207 us (1145 MB
+// at 5.5 TB/s); one over 100000 75 us; 4 tokens at 2048, 12 x 64, 8.7 us, two
 // launches of dependent rounds.
 #include <limits.h>
 

@@ -21,9 +21,9 @@
 //
 // Bound by the matrix cores together with the softmax's vector instructions and
 // the issue of the loads: on MI355X two chunks of 4096 bfloat16 tokens, 32 heads
-// over 8 x 128, 560 us or 960 TFLOP/s (an 8192^3 library product: 1230); 12 x 64
-// 83 us, 620 TFLOP/s (half the products per exponential), with capped scores
-// 131.  Without the next tile's loads 410 of 548 us, without the softmax 477,
+// over 8 x 128, 550 to 575 us or 935 to 980 TFLOP/s (an 8192^3 library product:
+// 1230); 12 x 64 83 us, 620 TFLOP/s (half the products per exponential), with
+// capped scores 131.  Without the next tile's loads 410 of 548 us, without the softmax 477,
 // products and LDS reads alone 326.
 //
 // Rows of K and V in LDS are as they lie in the pool, except that the 16-byte
